@@ -1,0 +1,366 @@
+// Backward of attention with a learned relative position bias.  With p from the forward pass's maximum and sum:
+//     dp_ij = grad_i . v_j      ds_ij = p_ij (dp_ij - delta_i)      delta_i = out_i . grad_i
+//     dq_i = scale sum_j ds_ij k_j     dk_j = scale sum_i ds_ij q_i     dv_j = sum_i p_ij grad_i
+//     dtable[u][h] = sum of ds over sequences and over the pairs of bucket u
+// Three kernels in the forward's form, each recomputing the scores: queries stay (dq, and delta for the others), keys stay
+// (dk, dv), and a tile of pairs stays while the batch streams past it (the table).  No sum crosses workgroups except the
+// table's, whose partial sums a last kernel adds in a fixed order.
+#include "attention.h"
+
+namespace ta_nn {
+
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* ks = reinterpret_cast<T*>(smem);
+    T* vs = ks + 64 * Tile<T, DP>::LD;
+    float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
+    const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
+    const int group = a.heads / a.kv_heads;
+    const int tiles = (a.m + 63) / 64;
+    const int64_t block = blockIdx.x;
+    const int i0 = static_cast<int>(block % tiles) * 64;
+    const int head = static_cast<int>(block / tiles % a.heads);
+    const int64_t b = block / tiles / a.heads;
+    const int hk = head / group;
+    const int start = a.query_start ? a.query_start[b] : a.start;
+    int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
+    if (a.causal) {
+        const int64_t last = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
+        keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
+    }
+    if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
+    const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
+
+    const bool valid = i0 + 16 * wave + c < a.m;
+    const int query = min(i0 + 16 * wave + c, a.m - 1);
+    const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
+    const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
+    const T* op = static_cast<const T*>(a.out) + b * a.o_sb + head * a.o_sh + query * a.o_sm;
+    typename Frag<T>::Row q[DC], go[DC];
+    float delta = 0.0f;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc) {
+        q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
+        go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
+        const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
+        const Vec<T> gv = __builtin_bit_cast(Vec<T>, go[dc]);
+#pragma unroll
+        for (int i = 0; i < Frag<T>::VE; ++i) delta += to_float(o.v[i]) * to_float(gv.v[i]);
+    }
+    delta += lane_xor(delta, 16);
+    delta += lane_xor(delta, 32);
+    const int64_t at = (b * a.heads + head) * a.m + query;
+    if (valid && g == 0) a.delta[at] = delta;
+    const float top = a.stats[2 * at], inv = a.stats[2 * at + 1];
+
+    f32x4 dq[1][DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    Staged<T, DP, 64, 256> kr, vr;
+    auto fetch = [&](int j0) {
+        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
+        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+    };
+    if (keys > 0) fetch(0);
+    for (int j0 = 0; j0 < keys; j0 += 64) {
+        __syncthreads();
+        kr.put(ks);
+        vr.put(vs);
+        __syncthreads();
+        if (j0 + 64 < keys) fetch(j0 + 64);
+        f32x4 s[4], ds[1][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+                s[t] = mma_row(row_frag<T, DP>(ks, 16 * t + c, dc, g), q[dc], s[t]);
+                ds[0][t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], ds[0][t]);
+            }
+        }
+        score_column(a, bias, b, query, start, j0, keys, g, s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = exp2_hw((s[t][r] - top) * kLog2e) * inv;
+                ds[0][t][r] = p == 0.0f ? 0.0f : p * (ds[0][t][r] - delta);       // a masked value may be anything
+            }
+        mma_transposed<DP, 1, 4>(ks, ds, dq, c, g);
+    }
+    if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* qs = reinterpret_cast<T*>(smem);
+    T* gs = qs + 64 * Tile<T, DP>::LD;
+    float* row_top = reinterpret_cast<float*>(gs + 64 * Tile<T, DP>::LD);
+    float* row_inv = row_top + 64;
+    float* row_delta = row_inv + 64;
+    float* bias_lds = row_delta + 64;
+    const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
+    const int group = a.heads / a.kv_heads;
+    const int tiles = (a.n + 63) / 64;
+    const int64_t block = blockIdx.x;
+    const int j0 = static_cast<int>(block % tiles) * 64;
+    const int hk = static_cast<int>(block / tiles % a.kv_heads);
+    const int64_t b = block / tiles / a.kv_heads;
+    const int start = a.query_start ? a.query_start[b] : a.start;
+    const int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
+    const bool valid = j0 + 16 * wave + c < a.n;
+    const int key = min(j0 + 16 * wave + c, a.n - 1);
+    const bool used = valid && key < keys;
+
+    typename Frag<T>::Row k[DC], v[DC];
+    const T* kp = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh + static_cast<int64_t>(key) * a.k_sn;
+    const T* vp = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh + static_cast<int64_t>(key) * a.v_sn;
+#pragma unroll
+    for (int dc = 0; dc < DC; ++dc) {
+        k[dc] = row_frag_global<T>(kp, a.dim, dc, g, used);
+        v[dc] = row_frag_global<T>(vp, a.dim, dc, g, used);
+    }
+    f32x4 dk[1][DT], dv[1][DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // the first query that sees any key of the block
+    const int i_first = a.causal ? max(0, clamp_token(static_cast<int64_t>(j0) - start)) / 64 * 64 : 0;
+    const int rows = j0 < keys ? max(0, a.m - i_first) : 0;
+    const int steps = (rows + 63) / 64;                  // per head of the group
+    Staged<T, DP, 64, 256> qr, gr;
+    float st_top = 0.0f, st_inv = 0.0f, st_delta = 0.0f;
+    auto fetch = [&](int step) {
+        const int head = hk * group + step / steps, i0 = i_first + step % steps * 64;
+        const T* q_base = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh;
+        const T* g_base = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh;
+        qr.load([&](int r) { return q_base + static_cast<int64_t>(i0 + r) * a.q_sm; }, a.m - i0, a.dim);
+        gr.load([&](int r) { return g_base + static_cast<int64_t>(i0 + r) * a.g_sm; }, a.m - i0, a.dim);
+        if (tid < 64) {
+            const bool in = i0 + tid < a.m;
+            const int64_t at = (b * a.heads + head) * a.m + min(i0 + tid, a.m - 1);
+            st_top = in ? a.stats[2 * at] : 0.0f;
+            st_inv = in ? a.stats[2 * at + 1] : 0.0f;
+            st_delta = in ? a.delta[at] : 0.0f;
+        }
+    };
+    if (steps > 0) fetch(0);
+    for (int step = 0; step < steps * group; ++step) {
+        const int head = hk * group + step / steps, i0 = i_first + step % steps * 64;
+        __syncthreads();
+        qr.put(qs);
+        gr.put(gs);
+        if (tid < 64) {
+            row_top[tid] = st_top;
+            row_inv[tid] = st_inv;
+            row_delta[tid] = st_delta;
+        }
+        if (a.bias_in_lds && step % steps == 0) stage_bias(a, bias_lds, head, 1, 256);
+        __syncthreads();
+        if (step + 1 < steps * group) fetch(step + 1);
+        f32x4 p[1][4], ds[1][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            p[0][t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+                p[0][t] = mma_row(row_frag<T, DP>(qs, 16 * t + c, dc, g), k[dc], p[0][t]);
+                ds[0][t] = mma_row(row_frag<T, DP>(gs, 16 * t + c, dc, g), v[dc], ds[0][t]);
+            }
+        }
+        const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
+        score_row(a, bias, b, key, start, i0, used, g, p[0]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const f32x4 top = *reinterpret_cast<const f32x4*>(row_top + 16 * t + 4 * g);
+            const f32x4 inv = *reinterpret_cast<const f32x4*>(row_inv + 16 * t + 4 * g);
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = exp2_hw((p[0][t][r] - top[r]) * kLog2e) * inv[r];
+                p[0][t][r] = w;
+                ds[0][t][r] = w == 0.0f ? 0.0f : w * (ds[0][t][r] - delta[r]);
+            }
+        }
+        mma_transposed<DP, 1, 4>(gs, p, dv, c, g);
+        mma_transposed<DP, 1, 4>(qs, ds, dk, c, g);
+    }
+    if (valid) {
+        store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + static_cast<int64_t>(key) * a.dk_sn, dk[0], a.scale, a.dim, g);
+        store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + static_cast<int64_t>(key) * a.dv_sn, dv[0], 1.0f, a.dim, g);
+    }
+}
+
+// ds of one tile of 64 queries x 64 keys of a head, summed over the sequences of a chunk.  Pairs: the tile as it is; distances:
+// its 127 diagonals (the distance is the same along each).
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attention_bwd_table(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* ks = reinterpret_cast<T*>(smem);
+    T* vs = ks + 64 * Tile<T, DP>::LD;
+    float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
+    const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
+    const int group = a.heads / a.kv_heads;
+    const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64;
+    const int64_t block = blockIdx.x;
+    const int k_tile = static_cast<int>(block % k_tiles), q_tile = static_cast<int>(block / k_tiles % q_tiles);
+    const int head = static_cast<int>(block / k_tiles / q_tiles % a.heads);
+    const int chunk = static_cast<int>(block / k_tiles / q_tiles / a.heads);
+    const int i0 = q_tile * 64, j0 = k_tile * 64, hk = head / group;
+    const bool valid = i0 + 16 * wave + c < a.m;
+    const int query = min(i0 + 16 * wave + c, a.m - 1);
+    if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
+    const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
+    f32x4 sum[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int b0 = static_cast<int>(static_cast<int64_t>(a.batch) * chunk / a.chunks);
+    const int b1 = static_cast<int>(static_cast<int64_t>(a.batch) * (chunk + 1) / a.chunks);
+    for (int64_t b = b0; b < b1; ++b) {
+        const int start = a.query_start ? a.query_start[b] : a.start;
+        int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
+        if (a.causal) {
+            const int64_t last = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
+            keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
+        }
+        if (j0 >= keys) continue;                        // (the same for the whole workgroup)
+        const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+        const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+        Staged<T, DP, 64, 256> kr, vr;
+        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
+        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+        const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
+        const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
+        typename Frag<T>::Row q[DC], go[DC];
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+            q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
+            go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
+        }
+        const int64_t at = (b * a.heads + head) * a.m + query;
+        const float top = a.stats[2 * at], inv = valid ? a.stats[2 * at + 1] : 0.0f, delta = a.delta[at];
+        __syncthreads();
+        kr.put(ks);
+        vr.put(vs);
+        __syncthreads();
+        f32x4 s[4], dp[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            s[t] = dp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+                s[t] = mma_row(row_frag<T, DP>(ks, 16 * t + c, dc, g), q[dc], s[t]);
+                dp[t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], dp[t]);
+            }
+        }
+        score_column(a, bias, b, query, start, j0, keys, g, s);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = valid ? exp2_hw((s[t][r] - top) * kLog2e) * inv : 0.0f;
+                sum[t][r] += p == 0.0f ? 0.0f : p * (dp[t][r] - delta);
+            }
+    }
+    if (a.distances == 0) {
+        float* out = a.partial + ((static_cast<int64_t>(chunk) * a.heads + head) * a.m + query) * a.n;
+        if (valid)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (j0 + 16 * t + 4 * g + r < a.n) out[j0 + 16 * t + 4 * g + r] = sum[t][r];
+        return;
+    }
+    __syncthreads();                                     // the tiles are read: their place holds the sums now, [key][query]
+    float* tile = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tile[(16 * t + 4 * g + r) * 65 + 16 * wave + c] = sum[t][r];
+    __syncthreads();
+    if (tid < 128) {
+        const int diagonal = tid - 63;                   // key - query
+        float total = 0.0f;
+        if (tid < 127)
+            for (int i = max(0, -diagonal); i < 64 - max(0, diagonal); ++i) total += tile[(i + diagonal) * 65 + i];
+        a.partial[(((static_cast<int64_t>(chunk) * a.heads + head) * q_tiles + q_tile) * k_tiles + k_tile) * 128 + tid] = total;
+    }
+}
+
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+    if (dtype == TA_NN_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == TA_NN_BF16) static_cast<bf16*>(p)[i] = from_float<bf16>(v);
+    else static_cast<fp16*>(p)[i] = from_float<fp16>(v);
+}
+
+// one workgroup for each bucket and head: the chunks' partial sums in a fixed order, in 64 bits
+__global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
+    __shared__ double red[4];
+    const int bucket = static_cast<int>(blockIdx.x) / a.heads, head = static_cast<int>(blockIdx.x) % a.heads;
+    double sum = 0.0;
+    if (a.distances == 0) {
+        const int64_t pairs = static_cast<int64_t>(a.m) * a.n;
+        const int from = a.pair_starts[bucket], count = a.pair_starts[bucket + 1] - from;
+        for (int64_t e = threadIdx.x; e < static_cast<int64_t>(count) * a.chunks; e += 256) {
+            const int64_t chunk = e / count;
+            sum += a.partial[(chunk * a.heads + head) * pairs + a.pair_order[from + e % count]];
+        }
+    } else {
+        const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64;
+        const int64_t entries = static_cast<int64_t>(q_tiles) * k_tiles * 128;
+        for (int64_t e = threadIdx.x; e < entries; e += 256) {
+            const int t = static_cast<int>(e & 127), k_tile = static_cast<int>(e / 128 % k_tiles), q_tile = static_cast<int>(e / 128 / k_tiles);
+            const int64_t d = static_cast<int64_t>(k_tile - q_tile) * 64 + t - 63 - a.start - a.first;
+            const int at = d < 0 ? 0 : d >= a.distances ? a.distances - 1 : static_cast<int>(d);
+            if (static_cast<const int*>(a.index)[at] != bucket) continue;
+            for (int chunk = 0; chunk < a.chunks; ++chunk) sum += a.partial[(static_cast<int64_t>(chunk) * a.heads + head) * entries + e];
+        }
+    }
+    sum = block_sum<4>(sum, red);
+    if (threadIdx.x == 0) store_as(a.dtable, static_cast<int64_t>(bucket) * a.heads + head, a.table_dtype, static_cast<float>(sum));
+}
+
+template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) {
+    const size_t tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
+    const size_t bias = bias_lds_bytes(a, 1);
+    const int64_t q_blocks = ceil_div(a.m, 64) * a.heads * a.batch, k_blocks = ceil_div(a.n, 64) * a.kv_heads * a.batch;
+    const int64_t t_blocks = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads * a.chunks;
+    TA_NN_REQUIRE(q_blocks <= 0x7FFFFFFF && k_blocks <= 0x7FFFFFFF && t_blocks <= 0x7FFFFFFF, "too many tokens for one launch");
+    hipLaunchKernelGGL((attention_bwd_q<T, DP>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a);
+    hipLaunchKernelGGL((attention_bwd_kv<T, DP>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), tiles + 3 * 64 * 4 + bias, st, a);
+    if (a.dtable) {
+        const size_t diagonals = 64 * 65 * 4;
+        hipLaunchKernelGGL((attention_bwd_table<T, DP>), dim3(static_cast<unsigned>(t_blocks)), dim3(256),
+                           (tiles + bias > diagonals ? tiles + bias : diagonals), st, a);
+        hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
+    }
+    return check_launch("ta_nn_attention_backward");
+}
+
+}  // namespace ta_nn
+
+extern "C" int ta_nn_attention_backward(const ta_nn_attention_args* args, void* stream) {
+    ta_nn::AttentionArgs a{};
+    if (int rc = ta_nn::check_attention(args, a)) return rc;
+    TA_NN_REQUIRE(a.grad && a.stats && a.dq && a.dk && a.dv && a.workspace, "null pointer");
+    if (a.distances == 0) {
+        TA_NN_REQUIRE(a.index_t && a.index_t_stride >= a.m && a.index_t_stride % 4 == 0 && reinterpret_cast<uintptr_t>(a.index_t) % 8 == 0,
+                      "transposed index stride %lld of %d queries", static_cast<long long>(a.index_t_stride), a.m);
+        TA_NN_REQUIRE(!a.dtable || (a.pair_order && a.pair_starts), "null pointer");
+        TA_NN_REQUIRE(!a.dtable || static_cast<int64_t>(a.m) * a.n < 0x7FFFFFFF, "%d x %d pairs", a.m, a.n);
+    }
+    TA_NN_REQUIRE(!(a.dtable && a.query_start && a.distances), "the table's gradient needs one position of query 0 for all sequences");
+    TA_NN_REQUIRE(static_cast<int64_t>(a.buckets) * a.heads <= 0x7FFFFFFF, "%d buckets, %d heads", a.buckets, a.heads);
+    a.delta = a.workspace;
+    a.partial = a.workspace + static_cast<int64_t>(a.batch) * a.heads * a.m;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    TA_NN_BY_TYPE_AND_DIM(a.dtype, a.dim, (ta_nn::launch_backward<T, DP>(a, st)));
+}

@@ -1,0 +1,153 @@
+// Attention with a learned relative position bias, forward (see attention.h for the formulas and the layout).
+#include "attention.h"
+
+namespace ta_nn {
+
+// One workgroup: 64 NQ columns (queries; those of all heads that share a key head in one row, so that shared heads share the
+// tiles) against every key they see, 64 at a time.
+template <class T, int DP, int NQ>
+__global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* ks = reinterpret_cast<T*>(smem);
+    T* vs = ks + 64 * Tile<T, DP>::LD;
+    float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
+    const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
+    const int group = a.heads / a.kv_heads;
+    const int64_t columns = static_cast<int64_t>(group) * a.m;
+    const int col_tiles = static_cast<int>((columns + 64 * NQ - 1) / (64 * NQ));
+    const int64_t block = blockIdx.x;
+    const int tile = static_cast<int>(block % col_tiles);
+    const int hk = static_cast<int>(block / col_tiles % a.kv_heads);
+    const int64_t b = block / col_tiles / a.kv_heads;
+
+    const int64_t col0 = static_cast<int64_t>(tile) * 64 * NQ;
+    const int64_t col1 = min(col0 + 64 * NQ, columns) - 1;
+    const int h0 = static_cast<int>(col0 / a.m), h1 = static_cast<int>(col1 / a.m);
+    const int start = a.query_start ? a.query_start[b] : a.start;
+    int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
+    if (a.causal) {
+        const int64_t last = static_cast<int64_t>(start) + (h0 == h1 ? col1 - static_cast<int64_t>(h1) * a.m : a.m - 1);
+        keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
+    }
+    if (a.bias_in_lds) stage_bias(a, bias_lds, hk * group + h0, h1 - h0 + 1, 256);
+
+    int head[NQ], query[NQ];
+    bool valid[NQ];
+    typename Frag<T>::Row q[NQ][DC];
+    f32x4 o[NQ][DT];
+    float m_run[NQ], l[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        const int64_t col = col0 + (wave * NQ + x) * 16 + c;
+        valid[x] = col < columns;
+        const int64_t at = valid[x] ? col : columns - 1;
+        const int h = static_cast<int>(at / a.m);
+        query[x] = static_cast<int>(at - static_cast<int64_t>(h) * a.m);
+        head[x] = hk * group + h;
+        const T* p = static_cast<const T*>(a.q) + b * a.q_sb + head[x] * a.q_sh + query[x] * a.q_sm;
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) q[x][dc] = row_frag_global<T>(p, a.dim, dc, g, valid[x]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[x][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m_run[x] = -INFINITY;
+        l[x] = 0.0f;
+    }
+    const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    Staged<T, DP, 64, 256> kr, vr;
+    auto fetch = [&](int j0) {
+        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
+        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+    };
+    if (keys > 0) fetch(0);
+    for (int j0 = 0; j0 < keys; j0 += 64) {
+        __syncthreads();
+        kr.put(ks);
+        vr.put(vs);
+        __syncthreads();
+        if (j0 + 64 < keys) fetch(j0 + 64);
+        f32x4 s[NQ][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int dc = 0; dc < DC; ++dc) {
+                const typename Frag<T>::Row kf = row_frag<T, DP>(ks, 16 * t + c, dc, g);
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+            const Bias bias{a, a.bias_in_lds ? bias_lds + (head[x] - hk * group - h0) * bias_entries(a) : nullptr, head[x]};
+            score_column(a, bias, b, query[x], start, j0, keys, g, s[x]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[x][t][r]);
+            top = fmaxf(top, lane_xor(top, 16));
+            top = fmaxf(top, lane_xor(top, 32));
+            const float m_new = fmaxf(m_run[x], top);
+            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float shrink = exp2_hw((m_run[x] - m_ref) * kLog2e);
+            m_run[x] = m_new;
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[x][t][r] = exp2_hw((s[x][t][r] - m_ref) * kLog2e);
+                    sum += s[x][t][r];
+                }
+            l[x] = l[x] * shrink + sum;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
+        }
+        mma_transposed<DP, NQ, 4>(vs, s, o, c, g);
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        float sum = l[x] + lane_xor(l[x], 16);
+        sum += lane_xor(sum, 32);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (!valid[x]) continue;
+        T* p = static_cast<T*>(a.out) + b * a.o_sb + head[x] * a.o_sh + query[x] * a.o_sm;
+        store_column<T, DP>(p, o[x], inv, a.dim, g);
+        if (a.stats && g == 0) {
+            float* st = a.stats + 2 * ((b * a.heads + head[x]) * a.m + query[x]);
+            st[0] = m_run[x] == -INFINITY ? 0.0f : m_run[x];
+            st[1] = inv;
+        }
+    }
+}
+
+template <class T, int DP> size_t forward_lds(AttentionArgs& a, int columns_of_block) {
+    const size_t tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
+    return tiles + bias_lds_bytes(a, columns_of_block);
+}
+
+template <class T, int DP> int launch_forward(AttentionArgs a, hipStream_t st) {
+    const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
+    const int64_t blocks = ceil_div(columns, 64) * a.kv_heads * a.batch;
+    TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
+    const size_t lds = forward_lds<T, DP>(a, 64);
+    hipLaunchKernelGGL((attention_fwd<T, DP, 1>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
+    return check_launch("ta_nn_attention");
+}
+
+}  // namespace ta_nn
+
+extern "C" int64_t ta_nn_attention_workspace(const ta_nn_attention_args* args, int backward) {
+    if (args == nullptr) return 0;
+    return ta_nn::workspace_floats(*args, backward != 0);
+}
+
+extern "C" int ta_nn_attention(const ta_nn_attention_args* args, void* stream) {
+    ta_nn::AttentionArgs a{};
+    if (int rc = ta_nn::check_attention(args, a)) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    TA_NN_BY_TYPE_AND_DIM(a.dtype, a.dim, (ta_nn::launch_forward<T, DP>(a, st)));
+}
