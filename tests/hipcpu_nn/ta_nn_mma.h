@@ -35,6 +35,7 @@ static inline unsigned long long __ballot(int pred) {
 namespace ta_nn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
@@ -48,9 +49,16 @@ template <class V> inline V lane_exchange(V v, int mask) {
     ta_nn_host::wave_sync();
     return r;
 }
-inline float lane_xor(float v, int mask) { return lane_exchange(v, mask); }
-inline int lane_xor(int v, int mask) { return lane_exchange(v, mask); }
-inline double lane_xor(double v, int mask) { return lane_exchange(v, mask); }
+template <class V, class Op> inline V reduce_rows(V v, Op op) {
+    v = op(v, lane_exchange(v, 16));
+    return op(v, lane_exchange(v, 32));
+}
+template <class V, class Op> inline V reduce_wave(V v, Op op) {
+    for (int mask = 1; mask < 16; mask <<= 1) v = op(v, lane_exchange(v, mask));
+    return reduce_rows(v, op);
+}
+inline void forget(u32x4&) {}
+inline float max_nan(float a, float b) { return a != a || b != b ? NAN : a > b ? a : b; }
 inline float exp2_hw(float x) { return x < -126.0f ? 0.0f : exp2f(x); }
 
 template <class Row, int PER> inline f32x4 mfma_any(Row a, Row b, f32x4 acc) {

@@ -62,18 +62,8 @@ template <class T, int DP, int ROWS, int THREADS> struct Staged {
         for (int i = 0; i < COUNT; ++i) {
             const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
             if ((ROWS * PER_ROW) % THREADS != 0 && e >= ROWS * PER_ROW) continue;
-            if (r < rows && d + VE <= dim) {
-                v[i] = load_vec(row_at(r) + d);
-            } else {
-#pragma unroll
-                for (int x = 0; x < VE; ++x) v[i].v[x] = from_float<T>(0.0f);
-                if (r < rows && d < dim) {
-                    const T* p = row_at(r) + d;
-#pragma unroll
-                    for (int x = 0; x < VE; ++x)
-                        if (d + x < dim) v[i].v[x] = p[x];
-                }
-            }
+            v[i].raw = u32x4{0, 0, 0, 0};
+            if (r < rows && d < dim) v[i] = load_part(row_at(r) + d, dim - d, 0u);
         }
     }
     __device__ __forceinline__ void put(T* lds) const {
@@ -95,12 +85,8 @@ template <class T, int DP> __device__ __forceinline__ typename Frag<T>::Row row_
 template <class T> __device__ __forceinline__ typename Frag<T>::Row row_frag_global(const T* p, int dim, int dc, int g, bool valid) {
     const int d = dc * Frag<T>::D + g * Frag<T>::VE;
     Vec<T> v;
-    if (valid && d + Frag<T>::VE <= dim) {
-        v = load_vec(p + d);
-    } else {
-#pragma unroll
-        for (int x = 0; x < Frag<T>::VE; ++x) v.v[x] = valid && d + x < dim ? p[d + x] : from_float<T>(0.0f);
-    }
+    v.raw = u32x4{0, 0, 0, 0};
+    if (valid && d < dim) v = load_part(p + d, dim - d, 0u);
     return __builtin_bit_cast(typename Frag<T>::Row, v);
 }
 

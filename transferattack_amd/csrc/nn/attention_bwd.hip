@@ -47,10 +47,9 @@ __global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
         const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
         const Vec<T> gv = __builtin_bit_cast(Vec<T>, go[dc]);
 #pragma unroll
-        for (int i = 0; i < Frag<T>::VE; ++i) delta += to_float(o.v[i]) * to_float(gv.v[i]);
+        for (int i = 0; i < Frag<T>::VE; ++i) delta += get(o, i) * get(gv, i);
     }
-    delta += lane_xor(delta, 16);
-    delta += lane_xor(delta, 32);
+    delta = reduce_rows(delta, Sum{});
     const int64_t at = (b * a.heads + head) * a.m + query;
     if (valid && g == 0) a.delta[at] = delta;
     const float top = a.stats[2 * at], inv = a.stats[2 * at + 1];

@@ -88,8 +88,7 @@ __global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, s[x][t][r]);
-            top = fmaxf(top, lane_xor(top, 16));
-            top = fmaxf(top, lane_xor(top, 32));
+            top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); });
             const float m_new = fmaxf(m_run[x], top);
             const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
             const float shrink = exp2_hw((m_run[x] - m_ref) * kLog2e);
@@ -110,8 +109,7 @@ __global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-        float sum = l[x] + lane_xor(l[x], 16);
-        sum += lane_xor(sum, 32);
+        const float sum = reduce_rows(l[x], Sum{});
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (!valid[x]) continue;
         T* p = static_cast<T*>(a.out) + b * a.o_sb + head[x] * a.o_sh + query[x] * a.o_sm;

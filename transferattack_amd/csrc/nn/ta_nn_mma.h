@@ -13,6 +13,7 @@
 namespace ta_nn {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
@@ -50,8 +51,70 @@ __device__ __forceinline__ float exp2_hw(float x) {
 #endif
 }
 
-__device__ __forceinline__ float lane_xor(float v, int mask) { return __shfl_xor(v, mask, 64); }
-__device__ __forceinline__ int lane_xor(int v, int mask) { return __shfl_xor(v, mask, 64); }
-__device__ __forceinline__ double lane_xor(double v, int mask) { return __shfl_xor(v, mask, 64); }
+// the same value, as far as the compiler is concerned another one: what was computed from it before is not kept for later
+__device__ __forceinline__ void forget(u32x4& v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(v));
+#endif
+}
+
+// the larger one, NaN if either is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_elementwise_maximum(a, b);
+#else
+    return a;
+#endif
+}
+
+// ---- all 64 lanes reduced to one value every lane has, in a fixed order, without LDS: within 16 lanes by DPP moves (the
+// neighbour, the other pair, then mirror images: what they meet is uniform by then), across by the row swaps of gfx950
+template <int CTRL, class V> __device__ __forceinline__ V dpp(V v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const unsigned lo = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u), CTRL, 0xF, 0xF, true));
+        const unsigned hi = static_cast<unsigned>(__builtin_amdgcn_mov_dpp(static_cast<int>(u >> 32), CTRL, 0xF, 0xF, true));
+        return __builtin_bit_cast(V, static_cast<uint64_t>(hi) << 32 | lo);
+    }
+#else
+    return v;
+#endif
+}
+// op(v of this row of 16 -- or half of 32 -- and of its neighbour), the same for both: rows 0 and 1, 2 and 3 / halves 0 and 1
+template <bool HALVES, class V, class Op> __device__ __forceinline__ V with_neighbour(V v, Op op) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto swap = [](unsigned x, unsigned (&r)[2]) {
+        const auto both = HALVES ? __builtin_amdgcn_permlane32_swap(x, x, false, false) : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        r[0] = both[0];
+        r[1] = both[1];
+    };
+    if constexpr (sizeof(V) == 4) {
+        unsigned r[2];
+        swap(__builtin_bit_cast(unsigned, v), r);
+        return op(__builtin_bit_cast(V, r[0]), __builtin_bit_cast(V, r[1]));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        unsigned lo[2], hi[2];
+        swap(static_cast<unsigned>(u), lo);
+        swap(static_cast<unsigned>(u >> 32), hi);
+        return op(__builtin_bit_cast(V, static_cast<uint64_t>(hi[0]) << 32 | lo[0]), __builtin_bit_cast(V, static_cast<uint64_t>(hi[1]) << 32 | lo[1]));
+    }
+#else
+    return v;
+#endif
+}
+template <class V, class Op> __device__ __forceinline__ V reduce_rows(V v, Op op) {       // across the four rows of 16 lanes only
+    return with_neighbour<true>(with_neighbour<false>(v, op), op);
+}
+template <class V, class Op> __device__ __forceinline__ V reduce_wave(V v, Op op) {
+    v = op(v, dpp<0xB1>(v));
+    v = op(v, dpp<0x4E>(v));
+    v = op(v, dpp<0x141>(v));
+    v = op(v, dpp<0x140>(v));
+    return reduce_rows(v, op);
+}
 
 }  // namespace ta_nn
