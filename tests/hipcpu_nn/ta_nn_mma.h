@@ -58,6 +58,7 @@ template <class V, class Op> inline V reduce_wave(V v, Op op) {
     return reduce_rows(v, op);
 }
 inline void forget(u32x4&) {}
+inline void order_memory() {}
 inline float max_nan(float a, float b) { return a != a || b != b ? NAN : a > b ? a : b; }
 inline float exp2_hw(float x) { return x < -126.0f ? 0.0f : exp2f(x); }
 
@@ -77,6 +78,15 @@ template <class Row, int PER> inline f32x4 mfma_any(Row a, Row b, f32x4 acc) {
     }
     ta_nn_host::wave_sync();
     return acc;
+}
+inline u16x4 read_transposed(const unsigned short* p) {
+    ta_nn_host::put(p);
+    ta_nn_host::wave_sync();
+    const int lane = threadIdx.x & 63, group = lane & 48, c = lane & 15;
+    u16x4 r;
+    for (int i = 0; i < 4; ++i) r[i] = ta_nn_host::get<const unsigned short*>(group + 4 * i + c / 4)[c % 4];
+    ta_nn_host::wave_sync();
+    return r;
 }
 inline f32x4 mfma(float a, float b, f32x4 c) { return mfma_any<float, 1>(a, b, c); }
 inline f32x4 mfma(half8 a, half8 b, f32x4 c) { return mfma_any<half8, 8>(a, b, c); }

@@ -3,8 +3,8 @@
 //     s_ij = scale q_i . k_j + table[bucket(i, j)][head] + mask_ij          over the keys j that query i sees
 //     p_ij = exp(s_ij - max_j s_ij) / sum_j exp(...)                        o_i = sum_j p_ij v_j
 //
-// Every kernel keeps one side -- the "columns", 16 to a wave -- in registers and streams the other -- the "rows", 64 to a
-// tile -- through LDS.  It computes D = rows x columns, so a lane holds four consecutive rows of ONE column: maxima, sums and
+// Every kernel keeps one side -- the "columns", 16 or 32 to a wave -- in registers and streams the other -- the "rows", 64 or
+// 32 to a tile -- through LDS.  It computes D = rows x columns, so a lane holds four consecutive rows of ONE column: maxima, sums and
 // rescaling are per lane, and D is by itself the B operand of the next product, which contracts over the rows
 // (O^T = V^T P^T and its like): probabilities never leave the registers.  For that product fp32 visits rows 4 g + r in step
 // r; 16-bit types visit rows 4 g + i and 16 + 4 g + i of 32 in one step.
@@ -45,6 +45,9 @@ __device__ __forceinline__ f32x4 mma_row(f32x4 a, f32x4 b, f32x4 c) {      // 16
 __device__ __forceinline__ f32x4 mma_row(bf16x8 a, bf16x8 b, f32x4 c) { return mfma(a, b, c); }
 __device__ __forceinline__ f32x4 mma_row(half8 a, half8 b, f32x4 c) { return mfma(a, b, c); }
 
+// rows of a tile over 16: as many as leave the accumulators their registers
+template <int DP> constexpr int kSubs = DP <= 64 ? 4 : 2;
+
 // LDS tile: ROWS rows of DP elements, rows 16 bytes longer than they need to be so that the 16 rows of a fragment start in
 // different banks
 template <class T, int DP> struct Tile {
@@ -53,25 +56,33 @@ template <class T, int DP> struct Tile {
 };
 
 // ROWS x DP elements from memory into registers (zero past `rows` and `dim`); `put` moves them to LDS one barrier later.
-// row_at(r): the pointer to row r (called for r < rows only)
+// `base`: row 0, the same for the workgroup; a row is less than 2^24 elements behind the last
 template <class T, int DP, int ROWS, int THREADS> struct Staged {
     static constexpr int VE = Frag<T>::VE, PER_ROW = DP / VE, COUNT = (ROWS * PER_ROW + THREADS - 1) / THREADS;
+    __device__ __forceinline__ static bool mine(int e) { return (ROWS * PER_ROW) % THREADS == 0 || e < ROWS * PER_ROW; }
     Vec<T> v[COUNT];
-    template <class RowAt> __device__ __forceinline__ void load(RowAt row_at, int rows, int dim) {
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dim) {
+        const int step = static_cast<int>(stride);
+        if (rows >= ROWS && dim == DP) {
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) {
-            const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
-            if ((ROWS * PER_ROW) % THREADS != 0 && e >= ROWS * PER_ROW) continue;
-            v[i].raw = u32x4{0, 0, 0, 0};
-            if (r < rows && d < dim) v[i] = load_part(row_at(r) + d, dim - d, 0u);
+            for (int i = 0; i < COUNT; ++i) {
+                const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
+                if (mine(e)) v[i] = load_vec(base + (r * step + d));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < COUNT; ++i) {
+                const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
+                v[i].raw = u32x4{0, 0, 0, 0};
+                if (mine(e) && r < rows && d < dim) v[i] = load_part(base + (r * step + d), dim - d);
+            }
         }
     }
     __device__ __forceinline__ void put(T* lds) const {
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) {
             const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
-            if ((ROWS * PER_ROW) % THREADS != 0 && e >= ROWS * PER_ROW) continue;
-            *reinterpret_cast<Vec<T>*>(lds + r * Tile<T, DP>::LD + d) = v[i];
+            if (mine(e)) *reinterpret_cast<Vec<T>*>(lds + r * Tile<T, DP>::LD + d) = v[i];
         }
     }
 };
@@ -86,7 +97,7 @@ template <class T> __device__ __forceinline__ typename Frag<T>::Row row_frag_glo
     const int d = dc * Frag<T>::D + g * Frag<T>::VE;
     Vec<T> v;
     v.raw = u32x4{0, 0, 0, 0};
-    if (valid && d < dim) v = load_part(p + d, dim - d, 0u);
+    if (valid && d < dim) v = load_part(p + d, dim - d);
     return __builtin_bit_cast(typename Frag<T>::Row, v);
 }
 
@@ -124,10 +135,10 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ
             for (int q = 0; q < NQ; ++q) b[q] = pack8(w[q][2 * s], w[q][2 * s + 1], T{});
 #pragma unroll
             for (int dt = 0; dt < DP / 16; ++dt) {
-                u16x8 a;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    a[i] = lds[(32 * s + (i & 4) * 4 + 4 * g + (i & 3)) * Tile<T, DP>::LD + 16 * dt + c].bits;
+                const unsigned short* p = reinterpret_cast<const unsigned short*>(lds) + (32 * s + 4 * g + (c >> 2)) * Tile<T, DP>::LD
+                                          + 16 * dt + 4 * (c & 3);
+                const u16x4 lo = read_transposed(p), hi = read_transposed(p + 16 * Tile<T, DP>::LD);
+                const u16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(__builtin_bit_cast(typename Frag<T>::Row, a), b[q], acc[q][dt]);
             }
@@ -136,32 +147,25 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ
 }
 
 // ---- bias and mask of a score
-// Values of the table for the heads [h0, h0 + count) in LDS: by bucket (pairs) or by distance.
-__device__ __forceinline__ int bias_entries(const AttentionArgs& a) { return a.distances ? a.distances : a.buckets; }
+// Scores are kept times log2 e, so that the exponential is one instruction: s' = (scale log2 e) q.k + (table log2 e) + mask log2 e.
+// The table's values for a block's heads stand in LDS, multiplied already, by bucket (pairs) or by distance; the latter with
+// its ends repeated kPad times, so that a tile that touches the range at all needs no clamping.
+constexpr int kPad = 192;                                // > 64 rows + 128 columns
+__host__ __device__ inline int bias_entries(const AttentionArgs& a) { return a.distances ? a.distances + 2 * kPad : a.buckets; }
+
+__device__ __forceinline__ float table_value(const AttentionArgs& a, int entry, int head) {
+    const int bucket = a.distances ? static_cast<const int*>(a.index)[entry] : entry;
+    return load_as_float(a.table, static_cast<int64_t>(bucket) * a.heads + head, a.table_dtype) * kLog2e;
+}
+__device__ __forceinline__ int clamp_distance(const AttentionArgs& a, int e) { return e < 0 ? 0 : e >= a.distances ? a.distances - 1 : e; }
 
 __device__ __forceinline__ void stage_bias(const AttentionArgs& a, float* lds, int h0, int count, int threads) {
     const int entries = bias_entries(a);
     for (int e = threadIdx.x; e < entries * count; e += threads) {
         const int h = e / entries, i = e % entries;
-        const int bucket = a.distances ? static_cast<const int*>(a.index)[i] : i;
-        lds[e] = load_as_float(a.table, static_cast<int64_t>(bucket) * a.heads + h0 + h, a.table_dtype);
+        lds[e] = table_value(a, a.distances ? clamp_distance(a, i - kPad) : i, h0 + h);
     }
 }
-
-// the table's values for one head, staged or in memory
-struct Bias {
-    const AttentionArgs& a;
-    const float* lds;
-    int head;
-    __device__ __forceinline__ float value(int entry) const {
-        if (lds) return lds[entry];
-        const int bucket = a.distances ? static_cast<const int*>(a.index)[entry] : entry;
-        return load_as_float(a.table, static_cast<int64_t>(bucket) * a.heads + head, a.table_dtype);
-    }
-    __device__ __forceinline__ float clamped(int entry) const {
-        return value(entry < 0 ? 0 : entry >= a.distances ? a.distances - 1 : entry);
-    }
-};
 
 // positions may lie anywhere: clamped to where adding a token's number (below 2^30) can neither overflow nor change the answer
 __device__ __forceinline__ int clamp_entry(int64_t e) {
@@ -171,62 +175,96 @@ __device__ __forceinline__ int clamp_token(int64_t t) {
     return static_cast<int>(max(static_cast<int64_t>(-1), min(t, static_cast<int64_t>(1) << 30)));
 }
 
-// a mask entry as what is added to the score.  The lowest finite values are raised to -1e38: nothing changes (a score vanishes
+// a mask entry as what is added to s'.  The lowest finite values are raised to -1e38: nothing changes (a score vanishes
 // beside either), and neither it nor its product with log2 e overflows.  -inf stays.
 __device__ __forceinline__ float mask_value(const AttentionArgs& a, int64_t at) {
     if (a.mask_kind == TA_NN_MASK_BOOL) return static_cast<const unsigned char*>(a.mask)[at] ? 0.0f : -INFINITY;
     const float f = load_as_float(a.mask, at, a.mask_kind - TA_NN_MASK_F32);
-    return f < -1e38f && f != -INFINITY ? -1e38f : f;
+    return (f < -1e38f && f != -INFINITY ? -1e38f : f) * kLog2e;
 }
 __device__ __forceinline__ float masked(float s, float add) { return add == -INFINITY ? -INFINITY : s + add; }   // whatever s is
 
-
-// scale, bias and mask of the scores of one column (a query) against keys j0 + 16 t + 4 g + r
-__device__ __forceinline__ void score_column(const AttentionArgs& a, const Bias& bias, int64_t b, int query, int start, int j0, int keys,
-                                             int g, f32x4 (&s)[4]) {
+// What one lane knows of its column: a query against a tile of keys, or a key against a tile of queries.
+struct Column {
+    const float* bias;                                   // its head's values in LDS, or null: the table is read in memory
+    int head;
+    int from;                                            // distances: entry of row 0; rows count up (keys) or down (queries)
+    int bound;                                           // rows seen: <= bound (keys), >= bound (queries)
+    const unsigned short* pairs;                         // pairs: the column's row of the index
+    int64_t mask;                                        // offset of row 0
+};
+__device__ __forceinline__ Column query_column(const AttentionArgs& a, const float* bias, int64_t b, int head, int query, int start,
+                                               int keys) {
     const int64_t position = static_cast<int64_t>(start) + query;
-    const int from = clamp_entry(-position - a.first);
-    const int last = a.causal ? min(clamp_token(position), keys - 1) : keys - 1;
-    const int64_t mask_row = a.mask_kind ? b % a.mask_period * a.mask_sb + bias.head * a.mask_sh + query * a.mask_sm : 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int j = j0 + 16 * t + 4 * g;
-        u16x4 bucket{0, 0, 0, 0};
-        if (a.distances == 0 && j < a.n)
-            bucket = *reinterpret_cast<const u16x4*>(static_cast<const unsigned short*>(a.index) + query * a.index_stride + j);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float f = -INFINITY;
-            if (j + r <= last) {
-                f = s[t][r] * a.scale + (a.distances ? bias.clamped(j + r + from) : bias.value(bucket[r]));
-                if (a.mask_kind) f = masked(f, mask_value(a, mask_row + (j + r) * a.mask_sn));
-            }
-            s[t][r] = f;
-        }
-    }
+    return Column{bias, head, clamp_entry(-position - a.first), a.causal ? min(clamp_token(position), keys - 1) : keys - 1,
+                  a.distances ? nullptr : static_cast<const unsigned short*>(a.index) + query * a.index_stride,
+                  a.mask_kind ? b % a.mask_period * a.mask_sb + head * a.mask_sh + query * a.mask_sm : 0};
+}
+__device__ __forceinline__ Column key_column(const AttentionArgs& a, const float* bias, int64_t b, int head, int key, int start) {
+    const int64_t lead = static_cast<int64_t>(key) - start;
+    return Column{bias, head, clamp_entry(lead - a.first), a.causal ? clamp_token(lead) : 0,
+                  a.distances ? nullptr : static_cast<const unsigned short*>(a.index_t) + key * a.index_t_stride,
+                  a.mask_kind ? b % a.mask_period * a.mask_sb + head * a.mask_sh + key * a.mask_sn : 0};
 }
 
-// the same for one column that is a key (one in use) against queries i0 + 16 t + 4 g + r
-__device__ __forceinline__ void score_row(const AttentionArgs& a, const Bias& bias, int64_t b, int key, int start, int i0, bool used, int g,
-                                          f32x4 (&s)[4]) {
-    const int64_t lead = static_cast<int64_t>(key) - start;
-    const int from = clamp_entry(lead - a.first);
-    const int first = a.causal ? clamp_token(lead) : 0;
-    const int64_t mask_at = a.mask_kind ? b % a.mask_period * a.mask_sb + bias.head * a.mask_sh + key * a.mask_sn : 0;
+// How a tile's scores are made, the same for the workgroup.  kConstant: every pair of the tile is seen and lies past the same end
+// of the distances; kNear: every pair is seen, distances come from LDS without clamping; kPairs: every pair is seen, buckets from
+// the index; kGeneral: anything.
+enum TileKind { kGeneral, kNear, kPairs, kLow, kHigh };
+
+// `low`, `high`: the lowest and the highest entry of the distances in the tile
+__device__ __forceinline__ TileKind tile_kind(const AttentionArgs& a, bool all_seen, bool one_head, int64_t low, int64_t high) {
+    if (a.mask_kind || !all_seen || !a.bias_in_lds) return kGeneral;
+    if (a.distances == 0) return kPairs;
+    if (high <= 0) return kLow;
+    if (low >= a.distances - 1) return kHigh;
+    return one_head ? kNear : kGeneral;
+}
+
+// s (q.k of rows row0 + 16 t + 4 g + r) -> s'; DOWN: rows are queries, whose distance falls as they rise
+template <bool DOWN, int SUBS>
+__device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column& col, TileKind kind, int row0, int g, f32x4 (&s)[SUBS]) {
+    const float c = a.scale * kLog2e;
+    if (kind == kLow || kind == kHigh) {
+        const float add = col.bias[kPad + (kind == kLow ? 0 : a.distances - 1)];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int i = i0 + 16 * t + 4 * g;
-        u16x4 bucket{0, 0, 0, 0};
-        if (a.distances == 0 && i < a.m && used)
-            bucket = *reinterpret_cast<const u16x4*>(static_cast<const unsigned short*>(a.index_t) + key * a.index_t_stride + i);
+        for (int t = 0; t < SUBS; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float f = -INFINITY;
-            if (used && i + r < a.m && i + r >= first) {
-                f = s[t][r] * a.scale + (a.distances ? bias.clamped(from - i - r) : bias.value(bucket[r]));
-                if (a.mask_kind) f = masked(f, mask_value(a, mask_at + (i + r) * a.mask_sm));
+            for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, add);
+    } else if (kind == kNear) {
+        const float* p = col.bias + kPad + (DOWN ? col.from - row0 - 4 * g : col.from + row0 + 4 * g);
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, p[DOWN ? -(16 * t + r) : 16 * t + r]);
+    } else if (kind == kPairs) {
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) {
+            const u16x4 bucket = *reinterpret_cast<const u16x4*>(col.pairs + row0 + 16 * t + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, col.bias[bucket[r]]);
+        }
+    } else {
+        const int rows = DOWN ? a.m : a.n;
+        const int64_t step = DOWN ? a.mask_sm : a.mask_sn;
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) {
+            order_memory();                              // not the loads of all four at once: that takes their addresses' registers
+            const int row = row0 + 16 * t + 4 * g;
+            u16x4 bucket{0, 0, 0, 0};
+            if (a.distances == 0 && row < rows) bucket = *reinterpret_cast<const u16x4*>(col.pairs + row);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float f = -INFINITY;
+                if (DOWN ? row + r < rows && row + r >= col.bound : row + r <= col.bound) {
+                    int e = bucket[r];
+                    if (a.distances) e = clamp_distance(a, DOWN ? col.from - row - r : col.from + row + r);
+                    const float add = col.bias ? col.bias[a.distances ? e + kPad : e] : table_value(a, e, col.head);
+                    f = fmaf(s[t][r], c, add);
+                    if (a.mask_kind) f = masked(f, mask_value(a, col.mask + (row + r) * step));
+                }
+                s[t][r] = f;
             }
-            s[t][r] = f;
         }
     }
 }
@@ -255,7 +293,7 @@ inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns) {
     const int64_t group = a.heads / a.kv_heads;
     int64_t spans = (columns - 1) / a.m + 2;
     if (spans > group) spans = group;
-    const int64_t bytes = spans * (a.distances ? a.distances : a.buckets) * 4;
+    const int64_t bytes = spans * bias_entries(a) * 4;
     a.bias_in_lds = bytes <= 24 * 1024;
     return a.bias_in_lds ? static_cast<size_t>(bytes) : 0;
 }

@@ -39,6 +39,9 @@ int check_attention(const ta_nn_attention_args* args, AttentionArgs& a) {
     }
     TA_NN_REQUIRE(a.mask_kind >= TA_NN_MASK_NONE && a.mask_kind <= TA_NN_MASK_F16, "mask kind %d", a.mask_kind);
     TA_NN_REQUIRE(a.mask_kind == TA_NN_MASK_NONE || (a.mask && a.mask_period >= 1), "mask period %d", a.mask_period);
+    const int64_t steps[] = {a.q_sm, a.k_sn, a.v_sn, a.g_sm};
+    for (int64_t step : steps)
+        TA_NN_REQUIRE(step > -(1 << 24) && step < (1 << 24), "token stride %lld (below 2^24 elements)", static_cast<long long>(step));
     a.chunks = table_chunks(a);
     return 0;
 }

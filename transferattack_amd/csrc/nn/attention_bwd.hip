@@ -10,19 +10,19 @@
 namespace ta_nn {
 
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+__global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 64 * Tile<T, DP>::LD;
-    float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
+    T* vs = ks + ROWS * Tile<T, DP>::LD;
+    float* bias_lds = reinterpret_cast<float*>(vs + ROWS * Tile<T, DP>::LD);
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int tiles = (a.m + 63) / 64;
-    const int64_t block = blockIdx.x;
-    const int i0 = static_cast<int>(block % tiles) * 64;
-    const int head = static_cast<int>(block / tiles % a.heads);
-    const int64_t b = block / tiles / a.heads;
+    const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.heads) * a.batch;     // as in attention_fwd
+    const int head = static_cast<int>(block % lanes % a.heads);
+    const int64_t b = block % lanes / a.heads;
+    const int i0 = (a.causal ? tiles - 1 - static_cast<int>(block / lanes) : static_cast<int>(block / lanes)) * 64;
     const int hk = head / group;
     const int start = a.query_start ? a.query_start[b] : a.start;
     int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
@@ -31,7 +31,6 @@ __global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
         keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
     }
     if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
-    const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
 
     const bool valid = i0 + 16 * wave + c < a.m;
     const int query = min(i0 + 16 * wave + c, a.m - 1);
@@ -53,27 +52,29 @@ __global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
     const int64_t at = (b * a.heads + head) * a.m + query;
     if (valid && g == 0) a.delta[at] = delta;
     const float top = a.stats[2 * at], inv = a.stats[2 * at + 1];
+    const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
+    const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
 
     f32x4 dq[1][DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
     const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    Staged<T, DP, 64, 256> kr, vr;
+    Staged<T, DP, ROWS, 256> kr, vr;
     auto fetch = [&](int j0) {
-        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
-        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+        kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
+        vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
     };
     if (keys > 0) fetch(0);
-    for (int j0 = 0; j0 < keys; j0 += 64) {
+    for (int j0 = 0; j0 < keys; j0 += ROWS) {
         __syncthreads();
         kr.put(ks);
         vr.put(vs);
         __syncthreads();
-        if (j0 + 64 < keys) fetch(j0 + 64);
-        f32x4 s[4], ds[1][4];
+        if (j0 + ROWS < keys) fetch(j0 + ROWS);
+        f32x4 s[SUBS], ds[1][SUBS];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < SUBS; ++t) {
             s[t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
@@ -81,36 +82,37 @@ __global__ __launch_bounds__(256) void attention_bwd_q(AttentionArgs a) {
                 ds[0][t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], ds[0][t]);
             }
         }
-        score_column(a, bias, b, query, start, j0, keys, g, s);
+        score_tile<false>(a, col, tile_kind(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), true,
+                                            j0 - pos1 - a.first, j0 + ROWS - 1 - pos0 - a.first), j0, g, s);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = exp2_hw((s[t][r] - top) * kLog2e) * inv;
+                const float p = exp2_hw(s[t][r] - top) * inv;
                 ds[0][t][r] = p == 0.0f ? 0.0f : p * (ds[0][t][r] - delta);       // a masked value may be anything
             }
-        mma_transposed<DP, 1, 4>(ks, ds, dq, c, g);
+        mma_transposed<DP, 1, SUBS>(ks, ds, dq, c, g);
     }
     if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+__global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* qs = reinterpret_cast<T*>(smem);
-    T* gs = qs + 64 * Tile<T, DP>::LD;
-    float* row_top = reinterpret_cast<float*>(gs + 64 * Tile<T, DP>::LD);
+    T* gs = qs + ROWS * Tile<T, DP>::LD;
+    float* row_top = reinterpret_cast<float*>(gs + ROWS * Tile<T, DP>::LD);
     float* row_inv = row_top + 64;
     float* row_delta = row_inv + 64;
     float* bias_lds = row_delta + 64;
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int tiles = (a.n + 63) / 64;
-    const int64_t block = blockIdx.x;
-    const int j0 = static_cast<int>(block % tiles) * 64;
-    const int hk = static_cast<int>(block / tiles % a.kv_heads);
-    const int64_t b = block / tiles / a.kv_heads;
+    const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.kv_heads) * a.batch;  // as in attention_fwd
+    const int hk = static_cast<int>(block % lanes % a.kv_heads);
+    const int64_t b = block % lanes / a.kv_heads;
+    const int j0 = static_cast<int>(block / lanes) * 64;
     const int start = a.query_start ? a.query_start[b] : a.start;
     const int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
     const bool valid = j0 + 16 * wave + c < a.n;
@@ -130,18 +132,18 @@ __global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
     for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     // the first query that sees any key of the block
-    const int i_first = a.causal ? max(0, clamp_token(static_cast<int64_t>(j0) - start)) / 64 * 64 : 0;
+    const int i_first = a.causal ? max(0, clamp_token(static_cast<int64_t>(j0) - start)) / ROWS * ROWS : 0;
     const int rows = j0 < keys ? max(0, a.m - i_first) : 0;
-    const int steps = (rows + 63) / 64;                  // per head of the group
-    Staged<T, DP, 64, 256> qr, gr;
+    const int steps = (rows + ROWS - 1) / ROWS;                  // per head of the group
+    Staged<T, DP, ROWS, 256> qr, gr;
     float st_top = 0.0f, st_inv = 0.0f, st_delta = 0.0f;
     auto fetch = [&](int step) {
-        const int head = hk * group + step / steps, i0 = i_first + step % steps * 64;
+        const int head = hk * group + step / steps, i0 = i_first + step % steps * ROWS;
         const T* q_base = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh;
         const T* g_base = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh;
-        qr.load([&](int r) { return q_base + static_cast<int64_t>(i0 + r) * a.q_sm; }, a.m - i0, a.dim);
-        gr.load([&](int r) { return g_base + static_cast<int64_t>(i0 + r) * a.g_sm; }, a.m - i0, a.dim);
-        if (tid < 64) {
+        qr.load(q_base + static_cast<int64_t>(i0) * a.q_sm, a.q_sm, a.m - i0, a.dim);
+        gr.load(g_base + static_cast<int64_t>(i0) * a.g_sm, a.g_sm, a.m - i0, a.dim);
+        if (tid < ROWS) {
             const bool in = i0 + tid < a.m;
             const int64_t at = (b * a.heads + head) * a.m + min(i0 + tid, a.m - 1);
             st_top = in ? a.stats[2 * at] : 0.0f;
@@ -151,11 +153,11 @@ __global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
     };
     if (steps > 0) fetch(0);
     for (int step = 0; step < steps * group; ++step) {
-        const int head = hk * group + step / steps, i0 = i_first + step % steps * 64;
+        const int head = hk * group + step / steps, i0 = i_first + step % steps * ROWS;
         __syncthreads();
         qr.put(qs);
         gr.put(gs);
-        if (tid < 64) {
+        if (tid < ROWS) {
             row_top[tid] = st_top;
             row_inv[tid] = st_inv;
             row_delta[tid] = st_delta;
@@ -163,9 +165,9 @@ __global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
         if (a.bias_in_lds && step % steps == 0) stage_bias(a, bias_lds, head, 1, 256);
         __syncthreads();
         if (step + 1 < steps * group) fetch(step + 1);
-        f32x4 p[1][4], ds[1][4];
+        f32x4 p[1][SUBS], ds[1][SUBS];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < SUBS; ++t) {
             p[0][t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
@@ -173,22 +175,29 @@ __global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
                 ds[0][t] = mma_row(row_frag<T, DP>(gs, 16 * t + c, dc, g), v[dc], ds[0][t]);
             }
         }
-        const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
-        score_row(a, bias, b, key, start, i0, used, g, p[0]);
+        const Column col = key_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, key, start);
+        // (a key out of use gets no gradient whatever its column holds: zeros are stored for it)
+        const int64_t lead0 = static_cast<int64_t>(j0) - start, lead1 = static_cast<int64_t>(min(j0 + 64, a.n)) - 1 - start;
+        score_tile<true>(a, col, tile_kind(a, i0 + ROWS <= a.m && (!a.causal || i0 >= lead1), true, lead0 - i0 - ROWS + 1 - a.first,
+                                           lead1 - i0 - a.first), i0, g, p[0]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < SUBS; ++t) {
             const f32x4 top = *reinterpret_cast<const f32x4*>(row_top + 16 * t + 4 * g);
             const f32x4 inv = *reinterpret_cast<const f32x4*>(row_inv + 16 * t + 4 * g);
             const f32x4 delta = *reinterpret_cast<const f32x4*>(row_delta + 16 * t + 4 * g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float w = exp2_hw((p[0][t][r] - top[r]) * kLog2e) * inv[r];
+                const float w = exp2_hw(p[0][t][r] - top[r]) * inv[r];
                 p[0][t][r] = w;
                 ds[0][t][r] = w == 0.0f ? 0.0f : w * (ds[0][t][r] - delta[r]);
             }
         }
-        mma_transposed<DP, 1, 4>(gs, p, dv, c, g);
-        mma_transposed<DP, 1, 4>(qs, ds, dk, c, g);
+        mma_transposed<DP, 1, SUBS>(gs, p, dv, c, g);
+        mma_transposed<DP, 1, SUBS>(qs, ds, dk, c, g);
+    }
+    if (!used) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if (valid) {
         store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + static_cast<int64_t>(key) * a.dk_sn, dk[0], a.scale, a.dim, g);
@@ -199,7 +208,7 @@ __global__ __launch_bounds__(256) void attention_bwd_kv(AttentionArgs a) {
 // ds of one tile of 64 queries x 64 keys of a head, summed over the sequences of a chunk.  Pairs: the tile as it is; distances:
 // its 127 diagonals (the distance is the same along each).
 template <class T, int DP>
-__global__ __launch_bounds__(256) void attention_bwd_table(AttentionArgs a) {
+__global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
@@ -216,7 +225,6 @@ __global__ __launch_bounds__(256) void attention_bwd_table(AttentionArgs a) {
     const bool valid = i0 + 16 * wave + c < a.m;
     const int query = min(i0 + 16 * wave + c, a.m - 1);
     if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
-    const Bias bias{a, a.bias_in_lds ? bias_lds : nullptr, head};
     f32x4 sum[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -233,8 +241,8 @@ __global__ __launch_bounds__(256) void attention_bwd_table(AttentionArgs a) {
         const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
         const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
         Staged<T, DP, 64, 256> kr, vr;
-        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
-        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+        kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
+        vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
         const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
         const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
         typename Frag<T>::Row q[DC], go[DC];
@@ -259,12 +267,15 @@ __global__ __launch_bounds__(256) void attention_bwd_table(AttentionArgs a) {
                 dp[t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], dp[t]);
             }
         }
-        score_column(a, bias, b, query, start, j0, keys, g, s);
+        const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
+        const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
+        score_tile<false>(a, col, tile_kind(a, j0 + 64 <= keys && (!a.causal || j0 + 63 <= pos0), true, j0 - pos1 - a.first,
+                                            j0 + 63 - pos0 - a.first), j0, g, s);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = valid ? exp2_hw((s[t][r] - top) * kLog2e) * inv : 0.0f;
+                const float p = valid ? exp2_hw(s[t][r] - top) * inv : 0.0f;
                 sum[t][r] += p == 0.0f ? 0.0f : p * (dp[t][r] - delta);
             }
     }
@@ -328,7 +339,7 @@ __global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
 }
 
 template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) {
-    const size_t tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
+    const size_t tiles = 2 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T), table_tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
     const size_t bias = bias_lds_bytes(a, 1);
     const int64_t q_blocks = ceil_div(a.m, 64) * a.heads * a.batch, k_blocks = ceil_div(a.n, 64) * a.kv_heads * a.batch;
     const int64_t t_blocks = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads * a.chunks;
@@ -338,7 +349,7 @@ template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) 
     if (a.dtable) {
         const size_t diagonals = 64 * 65 * 4;
         hipLaunchKernelGGL((attention_bwd_table<T, DP>), dim3(static_cast<unsigned>(t_blocks)), dim3(256),
-                           (tiles + bias > diagonals ? tiles + bias : diagonals), st, a);
+                           (table_tiles + bias > diagonals ? table_tiles + bias : diagonals), st, a);
         hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
     }
     return check_launch("ta_nn_attention_backward");

@@ -4,22 +4,27 @@
 namespace ta_nn {
 
 // One workgroup: 64 NQ columns (queries; those of all heads that share a key head in one row, so that shared heads share the
-// tiles) against every key they see, 64 at a time.
+// tiles) against every key they see, a tile at a time.
 template <class T, int DP, int NQ>
-__global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16;
+__global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + 64 * Tile<T, DP>::LD;
-    float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
+    T* vs = ks + ROWS * Tile<T, DP>::LD;
+    float* bias_lds = reinterpret_cast<float*>(vs + ROWS * Tile<T, DP>::LD);
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int64_t columns = static_cast<int64_t>(group) * a.m;
     const int col_tiles = static_cast<int>((columns + 64 * NQ - 1) / (64 * NQ));
-    const int64_t block = blockIdx.x;
-    const int tile = static_cast<int>(block % col_tiles);
-    const int hk = static_cast<int>(block / col_tiles % a.kv_heads);
-    const int64_t b = block / col_tiles / a.kv_heads;
+    // workgroups go to the XCDs in turn: with sequence and head as the fastest index an XCD's L2 holds few heads' keys and values
+    const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.kv_heads) * a.batch;
+    const int hk = static_cast<int>(block % lanes % a.kv_heads);
+    const int64_t b = block % lanes / a.kv_heads;
+    int tile = static_cast<int>(block / lanes);
+    if (a.causal) {                                      // the longest begin: the last queries of every head
+        const int per_head = col_tiles / group;
+        tile = per_head * group == col_tiles ? tile % group * per_head + per_head - 1 - tile / group : col_tiles - 1 - tile;
+    }
 
     const int64_t col0 = static_cast<int64_t>(tile) * 64 * NQ;
     const int64_t col1 = min(col0 + 64 * NQ, columns) - 1;
@@ -32,20 +37,22 @@ __global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
     }
     if (a.bias_in_lds) stage_bias(a, bias_lds, hk * group + h0, h1 - h0 + 1, 256);
 
-    int head[NQ], query[NQ];
+    int query[NQ];
     bool valid[NQ];
+    Column col[NQ];
     typename Frag<T>::Row q[NQ][DC];
     f32x4 o[NQ][DT];
     float m_run[NQ], l[NQ];
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-        const int64_t col = col0 + (wave * NQ + x) * 16 + c;
-        valid[x] = col < columns;
-        const int64_t at = valid[x] ? col : columns - 1;
-        const int h = static_cast<int>(at / a.m);
-        query[x] = static_cast<int>(at - static_cast<int64_t>(h) * a.m);
-        head[x] = hk * group + h;
-        const T* p = static_cast<const T*>(a.q) + b * a.q_sb + head[x] * a.q_sh + query[x] * a.q_sm;
+        const int64_t at = col0 + (wave * NQ + x) * 16 + c;
+        valid[x] = at < columns;
+        const int64_t own = valid[x] ? at : columns - 1;
+        const int h = static_cast<int>(own / a.m);
+        query[x] = static_cast<int>(own - static_cast<int64_t>(h) * a.m);
+        const int head = hk * group + h;
+        col[x] = query_column(a, a.bias_in_lds ? bias_lds + (h - h0) * bias_entries(a) : nullptr, b, head, query[x], start, keys);
+        const T* p = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query[x] * a.q_sm;
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc) q[x][dc] = row_frag_global<T>(p, a.dim, dc, g, valid[x]);
 #pragma unroll
@@ -53,23 +60,26 @@ __global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
         m_run[x] = -INFINITY;
         l[x] = 0.0f;
     }
+    // positions of the block's first and last query (of any, where it spans heads)
+    const int64_t pos0 = static_cast<int64_t>(start) + (h0 == h1 ? col0 - static_cast<int64_t>(h0) * a.m : 0);
+    const int64_t pos1 = static_cast<int64_t>(start) + (h0 == h1 ? col1 - static_cast<int64_t>(h1) * a.m : a.m - 1);
     const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
     const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    Staged<T, DP, 64, 256> kr, vr;
+    Staged<T, DP, ROWS, 256> kr, vr;
     auto fetch = [&](int j0) {
-        kr.load([&](int r) { return k_base + static_cast<int64_t>(j0 + r) * a.k_sn; }, keys - j0, a.dim);
-        vr.load([&](int r) { return v_base + static_cast<int64_t>(j0 + r) * a.v_sn; }, keys - j0, a.dim);
+        kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
+        vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
     };
     if (keys > 0) fetch(0);
-    for (int j0 = 0; j0 < keys; j0 += 64) {
+    for (int j0 = 0; j0 < keys; j0 += ROWS) {
         __syncthreads();
         kr.put(ks);
         vr.put(vs);
         __syncthreads();
-        if (j0 + 64 < keys) fetch(j0 + 64);
-        f32x4 s[NQ][4];
+        if (j0 + ROWS < keys) fetch(j0 + ROWS);
+        f32x4 s[NQ][SUBS];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < SUBS; ++t) {
 #pragma unroll
             for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -79,61 +89,64 @@ __global__ __launch_bounds__(256) void attention_fwd(AttentionArgs a) {
                 for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
             }
         }
+        const TileKind kind = tile_kind(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), h0 == h1, j0 - pos1 - a.first,
+                                        j0 + ROWS - 1 - pos0 - a.first);
 #pragma unroll
         for (int x = 0; x < NQ; ++x) {
-            const Bias bias{a, a.bias_in_lds ? bias_lds + (head[x] - hk * group - h0) * bias_entries(a) : nullptr, head[x]};
-            score_column(a, bias, b, query[x], start, j0, keys, g, s[x]);
+            score_tile<false>(a, col[x], kind, j0, g, s[x]);
             float top = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < SUBS; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, s[x][t][r]);
             top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); });
             const float m_new = fmaxf(m_run[x], top);
             const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float shrink = exp2_hw((m_run[x] - m_ref) * kLog2e);
+            const float shrink = exp2_hw(m_run[x] - m_ref);
             m_run[x] = m_new;
             float sum = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < SUBS; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[x][t][r] = exp2_hw((s[x][t][r] - m_ref) * kLog2e);
+                    s[x][t][r] = exp2_hw(s[x][t][r] - m_ref);
                     sum += s[x][t][r];
                 }
             l[x] = l[x] * shrink + sum;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
         }
-        mma_transposed<DP, NQ, 4>(vs, s, o, c, g);
+        mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
         const float sum = reduce_rows(l[x], Sum{});
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (!valid[x]) continue;
-        T* p = static_cast<T*>(a.out) + b * a.o_sb + head[x] * a.o_sh + query[x] * a.o_sm;
+        T* p = static_cast<T*>(a.out) + b * a.o_sb + col[x].head * a.o_sh + query[x] * a.o_sm;
         store_column<T, DP>(p, o[x], inv, a.dim, g);
         if (a.stats && g == 0) {
-            float* st = a.stats + 2 * ((b * a.heads + head[x]) * a.m + query[x]);
+            float* st = a.stats + 2 * ((b * a.heads + col[x].head) * a.m + query[x]);
             st[0] = m_run[x] == -INFINITY ? 0.0f : m_run[x];
             st[1] = inv;
         }
     }
 }
 
-template <class T, int DP> size_t forward_lds(AttentionArgs& a, int columns_of_block) {
-    const size_t tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
-    return tiles + bias_lds_bytes(a, columns_of_block);
+template <class T, int DP, int NQ> int launch_forward_by(AttentionArgs a, hipStream_t st) {
+    const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
+    const int64_t blocks = ceil_div(columns, 64 * NQ) * a.kv_heads * a.batch;
+    TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
+    const size_t lds = 2 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T) + bias_lds_bytes(a, 64 * NQ);
+    hipLaunchKernelGGL((attention_fwd<T, DP, NQ>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
+    return check_launch("ta_nn_attention");
 }
 
 template <class T, int DP> int launch_forward(AttentionArgs a, hipStream_t st) {
     const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
-    const int64_t blocks = ceil_div(columns, 64) * a.kv_heads * a.batch;
-    TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
-    const size_t lds = forward_lds<T, DP>(a, 64);
-    hipLaunchKernelGGL((attention_fwd<T, DP, 1>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
-    return check_launch("ta_nn_attention");
+    // 32 columns to a wave halve the LDS reads per product, which is what 16-bit products wait for; not where that leaves CUs idle
+    if (sizeof(T) == 2 && ceil_div(columns, 128) * a.kv_heads * a.batch >= 512) return launch_forward_by<T, DP, sizeof(T) == 2 ? 2 : 1>(a, st);
+    return launch_forward_by<T, DP, 1>(a, st);
 }
 
 }  // namespace ta_nn

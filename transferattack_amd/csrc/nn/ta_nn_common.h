@@ -84,13 +84,12 @@ template <class T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
     __builtin_memcpy(&r.raw, p, 16);
     return r;
 }
-// the first `count` elements at p (as many as there are), the rest `fill`
-template <class T> __device__ __forceinline__ Vec<T> load_part(const T* p, int count, unsigned fill) {
+// the first `count` elements at p (as many as there are), the rest 0
+template <class T> __device__ __forceinline__ Vec<T> load_part(const T* p, int count) {
     if (count >= Vec<T>::N) return load_vec(p);
-    Vec<T> r;
-    r.raw = u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) set_bits(r, i, i < count ? bits_of(p[i]) : fill);
+    Vec<T> r{u32x4{0, 0, 0, 0}};
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) set_bits_at(r, i, bits_of(p[i]));
     return r;
 }
 template <class T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) { __builtin_memcpy(p, &r.raw, 16); }
@@ -98,16 +97,6 @@ template <class T> __device__ __forceinline__ T element(const Vec<T>& v, int i) 
     if constexpr (sizeof(T) == 4) return __uint_as_float(v.raw[i]);
     else return T{static_cast<unsigned short>(i & 1 ? v.raw[i >> 1] >> 16 : v.raw[i >> 1])};
 }
-template <class T> __device__ __forceinline__ void store_part(T* p, int count, const Vec<T>& v) {
-    if (count >= Vec<T>::N) {
-        store_vec(p, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < Vec<T>::N; ++i)
-            if (i < count) p[i] = element(v, i);
-    }
-}
-
 // a scalar of a runtime type: 0 fp32, 1 bf16, 2 fp16 (TA_NN_F32 ...)
 __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
     if (dtype == TA_NN_F32) return static_cast<const float*>(p)[i];

@@ -42,6 +42,17 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 #endif
 }
 
+// Four rows of 16 16-bit elements of an LDS tile, transposed: lane c of each group of 16 gets element c of rows 0 .. 3.  Lane c
+// passes the address of row c / 4, elements 4 (c % 4) .. + 3 of the group's four rows; groups are independent.
+__device__ __forceinline__ u16x4 read_transposed(const unsigned short* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef short v4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4*)(p)));
+#else
+    return u16x4{0, 0, 0, 0};
+#endif
+}
+
 // 2^x by the hardware instruction (about 1 ulp; results below 2^-126 become 0), log2 likewise
 __device__ __forceinline__ float exp2_hw(float x) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -55,6 +66,13 @@ __device__ __forceinline__ float exp2_hw(float x) {
 __device__ __forceinline__ void forget(u32x4& v) {
 #if defined(__HIP_DEVICE_COMPILE__)
     asm volatile("" : "+v"(v));
+#endif
+}
+
+// loads and stores are not moved across
+__device__ __forceinline__ void order_memory() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" ::: "memory");
 #endif
 }
 

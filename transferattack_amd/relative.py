@@ -219,8 +219,7 @@ def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
         for t in (dq, dk, dv):
             t.zero_()
         return dtable
-    if grad.stride(-1) != 1:
-        grad = grad.contiguous()
+    grad = _dense_rows(grad)
     a = _arguments(q, k, v, table, out, stats, o)
     a.grad = grad.data_ptr()
     a.g_sb, a.g_sh, a.g_sm, _ = grad.stride()
@@ -287,8 +286,10 @@ class _PackedAttention(torch.autograd.Function):
         return dqkv, dtable, None, None
 
 
-def _dense_rows(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _dense_rows(t, token=2):
+    """as the kernels take it: the innermost dimension dense, tokens less than 2^24 elements apart"""
+    dense = (t.stride(-1) == 1 or t.shape[-1] == 1) and abs(t.stride(token)) < 1 << 24
+    return t if dense else t.contiguous()
 
 
 def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=False, key_lengths=None, query_start=0):
@@ -329,4 +330,4 @@ def relative_attention_packed(qkv, table, buckets, scale=None, mask=None, causal
     q = qkv.detach().select(2, 0).transpose(1, 2)
     o = _options(q, q, table, buckets, scale, mask, causal, key_lengths, 0)
     save = torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad)
-    return _PackedAttention.apply(_dense_rows(qkv), table.contiguous(), o, save)
+    return _PackedAttention.apply(_dense_rows(qkv, 1), table.contiguous(), o, save)
