@@ -207,37 +207,59 @@ __device__ __forceinline__ Column key_column(const AttentionArgs& a, const float
                   a.mask_kind ? b % a.mask_period * a.mask_sb + head * a.mask_sh + key * a.mask_sn : 0};
 }
 
-// How a tile's scores are made, the same for the workgroup.  kConstant: every pair of the tile is seen and lies past the same end
-// of the distances; kNear: every pair is seen, distances come from LDS without clamping; kPairs: every pair is seen, buckets from
-// the index; kGeneral: anything.
-enum TileKind { kGeneral, kNear, kPairs, kLow, kHigh };
+// How the scores of a tile are made.  A kernel is compiled for one of three Biases, so that none carries the registers of the
+// others; within it every tile has one Kind, the same for the workgroup, and the loop's body is compiled for each, without branches.
+enum Biases {
+    kByDistance,                                         // distances in LDS, no mask
+    kByPair,                                             // pairs, the table in LDS, no mask
+    kAny                                                 // anything: masks, tables too large for LDS
+};
+enum Kind {
+    kConstant,                                           // every pair is seen and lies past the same end of the distances
+    kNear,                                               // every pair is seen; distances from LDS without clamping
+    kSeen,                                               // every pair is seen; buckets from the index
+    kEdge                                                // whatever there is
+};
 
 // `low`, `high`: the lowest and the highest entry of the distances in the tile
-__device__ __forceinline__ TileKind tile_kind(const AttentionArgs& a, bool all_seen, bool one_head, int64_t low, int64_t high) {
-    if (a.mask_kind || !all_seen || !a.bias_in_lds) return kGeneral;
-    if (a.distances == 0) return kPairs;
-    if (high <= 0) return kLow;
-    if (low >= a.distances - 1) return kHigh;
-    return one_head ? kNear : kGeneral;
+template <int BIASES> __device__ __forceinline__ Kind tile_kind(const AttentionArgs& a, bool all_seen, bool one_head, int64_t low, int64_t high) {
+    if (BIASES == kAny || !all_seen) return kEdge;
+    if (BIASES == kByPair) return kSeen;
+    if (high <= 0 || low >= a.distances - 1) return kConstant;
+    return one_head ? kNear : kEdge;
+}
+
+template <int K> struct KindTag { static constexpr int kind = K; };
+// body(KindTag<..>) for the tile's kind
+template <int BIASES, class Body> __device__ __forceinline__ void by_kind(Kind kind, Body&& body) {
+    if constexpr (BIASES == kByDistance) {
+        if (kind == kConstant) return body(KindTag<kConstant>{});
+        if (kind == kNear) return body(KindTag<kNear>{});
+    }
+    if constexpr (BIASES == kByPair) {
+        if (kind == kSeen) return body(KindTag<kSeen>{});
+    }
+    body(KindTag<kEdge>{});
 }
 
 // s (q.k of rows row0 + 16 t + 4 g + r) -> s'; DOWN: rows are queries, whose distance falls as they rise
-template <bool DOWN, int SUBS>
-__device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column& col, TileKind kind, int row0, int g, f32x4 (&s)[SUBS]) {
+template <int BIASES, int KIND, bool DOWN, int SUBS>
+__device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column& col, int row0, int g, f32x4 (&s)[SUBS]) {
     const float c = a.scale * kLog2e;
-    if (kind == kLow || kind == kHigh) {
-        const float add = col.bias[kPad + (kind == kLow ? 0 : a.distances - 1)];
+    if constexpr (KIND == kConstant) {
+        const int at = DOWN ? col.from - row0 : col.from + row0;       // all on the same side of the range
+        const float add = col.bias[kPad + (at < a.distances / 2 ? 0 : a.distances - 1)];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, add);
-    } else if (kind == kNear) {
+    } else if constexpr (KIND == kNear) {
         const float* p = col.bias + kPad + (DOWN ? col.from - row0 - 4 * g : col.from + row0 + 4 * g);
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, p[DOWN ? -(16 * t + r) : 16 * t + r]);
-    } else if (kind == kPairs) {
+    } else if constexpr (KIND == kSeen) {
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             const u16x4 bucket = *reinterpret_cast<const u16x4*>(col.pairs + row0 + 16 * t + 4 * g);
@@ -247,23 +269,29 @@ __device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column&
     } else {
         const int rows = DOWN ? a.m : a.n;
         const int64_t step = DOWN ? a.mask_sm : a.mask_sn;
+        const bool distances = BIASES == kByDistance || (BIASES == kAny && a.distances != 0);
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
-            order_memory();                              // not the loads of all four at once: that takes their addresses' registers
+            if (BIASES == kAny) order_memory();          // not the loads of all at once: that takes their addresses' registers
             const int row = row0 + 16 * t + 4 * g;
             u16x4 bucket{0, 0, 0, 0};
-            if (a.distances == 0 && row < rows) bucket = *reinterpret_cast<const u16x4*>(col.pairs + row);
+            if (!distances && row < rows) bucket = *reinterpret_cast<const u16x4*>(col.pairs + row);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float f = -INFINITY;
-                if (DOWN ? row + r < rows && row + r >= col.bound : row + r <= col.bound) {
-                    int e = bucket[r];
-                    if (a.distances) e = clamp_distance(a, DOWN ? col.from - row - r : col.from + row + r);
-                    const float add = col.bias ? col.bias[a.distances ? e + kPad : e] : table_value(a, e, col.head);
-                    f = fmaf(s[t][r], c, add);
-                    if (a.mask_kind) f = masked(f, mask_value(a, col.mask + (row + r) * step));
+                const bool seen = DOWN ? row + r < rows && row + r >= col.bound : row + r <= col.bound;
+                int e = bucket[r];
+                if (distances) e = clamp_distance(a, DOWN ? col.from - row - r : col.from + row + r);
+                if constexpr (BIASES != kAny) {
+                    const float f = fmaf(s[t][r], c, col.bias[distances ? e + kPad : e]);
+                    s[t][r] = seen ? f : -INFINITY;
+                } else {
+                    float f = -INFINITY;
+                    if (seen) {
+                        f = fmaf(s[t][r], c, col.bias ? col.bias[distances ? e + kPad : e] : table_value(a, e, col.head));
+                        if (a.mask_kind) f = masked(f, mask_value(a, col.mask + (row + r) * step));
+                    }
+                    s[t][r] = f;
                 }
-                s[t][r] = f;
             }
         }
     }
@@ -298,10 +326,20 @@ inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns) {
     return a.bias_in_lds ? static_cast<size_t>(bytes) : 0;
 }
 
+inline int biases_of(const AttentionArgs& a) { return a.mask_kind || !a.bias_in_lds ? kAny : a.distances ? kByDistance : kByPair; }
+
 int check_attention(const ta_nn_attention_args* args, AttentionArgs& a);
 int64_t workspace_floats(const ta_nn_attention_args& a, bool backward);
 
 }  // namespace ta_nn
+
+// launch<.., BIASES>(...) for the call's biases
+#define TA_NN_BY_BIASES(a, call)                                          \
+    switch (ta_nn::biases_of(a)) {                                        \
+        case ta_nn::kByDistance: { constexpr int BIASES = ta_nn::kByDistance; call; break; } \
+        case ta_nn::kByPair: { constexpr int BIASES = ta_nn::kByPair; call; break; }         \
+        default: { constexpr int BIASES = ta_nn::kAny; call; break; }     \
+    }
 
 #define TA_NN_DIMS(call)                                                  \
     if (ta_nn_dim <= 32) { constexpr int DP = 32; return call; }          \

@@ -9,7 +9,7 @@
 
 namespace ta_nn {
 
-template <class T, int DP>
+template <class T, int DP, int BIASES>
 __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -72,6 +72,9 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
         vr.put(vs);
         __syncthreads();
         if (j0 + ROWS < keys) fetch(j0 + ROWS);
+        const Kind kind = tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), true, j0 - pos1 - a.first,
+                                            j0 + ROWS - 1 - pos0 - a.first);
+        by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 s[SUBS], ds[1][SUBS];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
@@ -82,8 +85,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
                 ds[0][t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], ds[0][t]);
             }
         }
-        score_tile<false>(a, col, tile_kind(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), true,
-                                            j0 - pos1 - a.first, j0 + ROWS - 1 - pos0 - a.first), j0, g, s);
+        score_tile<BIASES, decltype(tag)::kind, false>(a, col, j0, g, s);
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
@@ -92,11 +94,12 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
                 ds[0][t][r] = p == 0.0f ? 0.0f : p * (ds[0][t][r] - delta);       // a masked value may be anything
             }
         mma_transposed<DP, 1, SUBS>(ks, ds, dq, c, g);
+        });
     }
     if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
 }
 
-template <class T, int DP>
+template <class T, int DP, int BIASES>
 __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -165,6 +168,12 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
         if (a.bias_in_lds && step % steps == 0) stage_bias(a, bias_lds, head, 1, 256);
         __syncthreads();
         if (step + 1 < steps * group) fetch(step + 1);
+        const Column col = key_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, key, start);
+        // (a key out of use gets no gradient whatever its column holds: zeros are stored for it)
+        const int64_t lead0 = static_cast<int64_t>(j0) - start, lead1 = static_cast<int64_t>(min(j0 + 64, a.n)) - 1 - start;
+        const Kind kind = tile_kind<BIASES>(a, i0 + ROWS <= a.m && (!a.causal || i0 >= lead1), true, lead0 - i0 - ROWS + 1 - a.first,
+                                            lead1 - i0 - a.first);
+        by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 p[1][SUBS], ds[1][SUBS];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
@@ -175,11 +184,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
                 ds[0][t] = mma_row(row_frag<T, DP>(gs, 16 * t + c, dc, g), v[dc], ds[0][t]);
             }
         }
-        const Column col = key_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, key, start);
-        // (a key out of use gets no gradient whatever its column holds: zeros are stored for it)
-        const int64_t lead0 = static_cast<int64_t>(j0) - start, lead1 = static_cast<int64_t>(min(j0 + 64, a.n)) - 1 - start;
-        score_tile<true>(a, col, tile_kind(a, i0 + ROWS <= a.m && (!a.causal || i0 >= lead1), true, lead0 - i0 - ROWS + 1 - a.first,
-                                           lead1 - i0 - a.first), i0, g, p[0]);
+        score_tile<BIASES, decltype(tag)::kind, true>(a, col, i0, g, p[0]);
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             const f32x4 top = *reinterpret_cast<const f32x4*>(row_top + 16 * t + 4 * g);
@@ -194,6 +199,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
         }
         mma_transposed<DP, 1, SUBS>(gs, p, dv, c, g);
         mma_transposed<DP, 1, SUBS>(qs, ds, dk, c, g);
+        });
     }
     if (!used) {
 #pragma unroll
@@ -207,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
 
 // ds of one tile of 64 queries x 64 keys of a head, summed over the sequences of a chunk.  Pairs: the tile as it is; distances:
 // its 127 diagonals (the distance is the same along each).
-template <class T, int DP>
+template <class T, int DP, int BIASES>
 __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -257,6 +263,11 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
         kr.put(ks);
         vr.put(vs);
         __syncthreads();
+        const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
+        const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
+        const Kind kind = tile_kind<BIASES>(a, j0 + 64 <= keys && (!a.causal || j0 + 63 <= pos0), true, j0 - pos1 - a.first,
+                                            j0 + 63 - pos0 - a.first);
+        by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 s[4], dp[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -267,10 +278,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
                 dp[t] = mma_row(row_frag<T, DP>(vs, 16 * t + c, dc, g), go[dc], dp[t]);
             }
         }
-        const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
-        const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
-        score_tile<false>(a, col, tile_kind(a, j0 + 64 <= keys && (!a.causal || j0 + 63 <= pos0), true, j0 - pos1 - a.first,
-                                            j0 + 63 - pos0 - a.first), j0, g, s);
+        score_tile<BIASES, decltype(tag)::kind, false>(a, col, j0, g, s);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -278,6 +286,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
                 const float p = valid ? exp2_hw(s[t][r] - top) * inv : 0.0f;
                 sum[t][r] += p == 0.0f ? 0.0f : p * (dp[t][r] - delta);
             }
+        });
     }
     if (a.distances == 0) {
         float* out = a.partial + ((static_cast<int64_t>(chunk) * a.heads + head) * a.m + query) * a.n;
@@ -344,12 +353,12 @@ template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) 
     const int64_t q_blocks = ceil_div(a.m, 64) * a.heads * a.batch, k_blocks = ceil_div(a.n, 64) * a.kv_heads * a.batch;
     const int64_t t_blocks = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads * a.chunks;
     TA_NN_REQUIRE(q_blocks <= 0x7FFFFFFF && k_blocks <= 0x7FFFFFFF && t_blocks <= 0x7FFFFFFF, "too many tokens for one launch");
-    hipLaunchKernelGGL((attention_bwd_q<T, DP>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a);
-    hipLaunchKernelGGL((attention_bwd_kv<T, DP>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), tiles + 3 * 64 * 4 + bias, st, a);
+    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_q<T, DP, BIASES>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a));
+    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_kv<T, DP, BIASES>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), tiles + 3 * 64 * 4 + bias, st, a));
     if (a.dtable) {
         const size_t diagonals = 64 * 65 * 4;
-        hipLaunchKernelGGL((attention_bwd_table<T, DP>), dim3(static_cast<unsigned>(t_blocks)), dim3(256),
-                           (table_tiles + bias > diagonals ? table_tiles + bias : diagonals), st, a);
+        const size_t lds = table_tiles + bias > diagonals ? table_tiles + bias : diagonals;
+        TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_table<T, DP, BIASES>), dim3(static_cast<unsigned>(t_blocks)), dim3(256), lds, st, a));
         hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
     }
     return check_launch("ta_nn_attention_backward");

@@ -3,15 +3,17 @@
 
 namespace ta_nn {
 
+constexpr float kSlack = 8.0f;
+
 // One workgroup: 64 NQ columns (queries; those of all heads that share a key head in one row, so that shared heads share the
-// tiles) against every key they see, a tile at a time.
-template <class T, int DP, int NQ>
+// tiles) against every key they see, a tile at a time.  Two tiles in LDS: while one is worked on, the next arrives in registers
+// and is put into the other's place, with one barrier a tile.
+template <class T, int DP, int NQ, int BIASES>
 __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS, TILE = ROWS * Tile<T, DP>::LD;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* ks = reinterpret_cast<T*>(smem);
-    T* vs = ks + ROWS * Tile<T, DP>::LD;
-    float* bias_lds = reinterpret_cast<float*>(vs + ROWS * Tile<T, DP>::LD);
+    T* tiles = reinterpret_cast<T*>(smem);               // [2][keys, values][ROWS][LD]
+    float* bias_lds = reinterpret_cast<float*>(tiles + 4 * TILE);
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int64_t columns = static_cast<int64_t>(group) * a.m;
@@ -30,11 +32,21 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
     const int64_t col1 = min(col0 + 64 * NQ, columns) - 1;
     const int h0 = static_cast<int>(col0 / a.m), h1 = static_cast<int>(col1 / a.m);
     const int start = a.query_start ? a.query_start[b] : a.start;
+    // positions of the block's first and last query (of any, where it spans heads)
+    const int64_t pos0 = static_cast<int64_t>(start) + (h0 == h1 ? col0 - static_cast<int64_t>(h0) * a.m : 0);
+    const int64_t pos1 = static_cast<int64_t>(start) + (h0 == h1 ? col1 - static_cast<int64_t>(h1) * a.m : a.m - 1);
     int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
-    if (a.causal) {
-        const int64_t last = static_cast<int64_t>(start) + (h0 == h1 ? col1 - static_cast<int64_t>(h1) * a.m : a.m - 1);
-        keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
-    }
+    if (a.causal) keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), pos1 + 1)));
+
+    const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
+    const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
+    Staged<T, DP, ROWS, 256> kr, vr;
+    auto fetch = [&](int j0) {
+        if (j0 >= keys) return;
+        kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
+        vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
+    };
+    fetch(0);
     if (a.bias_in_lds) stage_bias(a, bias_lds, hk * group + h0, h1 - h0 + 1, 256);
 
     int query[NQ];
@@ -60,63 +72,78 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
         m_run[x] = -INFINITY;
         l[x] = 0.0f;
     }
-    // positions of the block's first and last query (of any, where it spans heads)
-    const int64_t pos0 = static_cast<int64_t>(start) + (h0 == h1 ? col0 - static_cast<int64_t>(h0) * a.m : 0);
-    const int64_t pos1 = static_cast<int64_t>(start) + (h0 == h1 ? col1 - static_cast<int64_t>(h1) * a.m : a.m - 1);
-    const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
-    const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    Staged<T, DP, ROWS, 256> kr, vr;
-    auto fetch = [&](int j0) {
-        kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
-        vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
-    };
-    if (keys > 0) fetch(0);
-    for (int j0 = 0; j0 < keys; j0 += ROWS) {
-        __syncthreads();
-        kr.put(ks);
-        vr.put(vs);
-        __syncthreads();
-        if (j0 + ROWS < keys) fetch(j0 + ROWS);
-        f32x4 s[NQ][SUBS];
+    if (keys > 0) {
+        kr.put(tiles);
+        vr.put(tiles + TILE);
+        fetch(ROWS);
+    }
+    __syncthreads();
+    for (int j0 = 0, turn = 0; j0 < keys; j0 += ROWS, turn ^= 1) {
+        const T* ks = tiles + turn * 2 * TILE;
+        const T* vs = ks + TILE;
+        by_kind<BIASES>(tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), h0 == h1, j0 - pos1 - a.first,
+                                          j0 + ROWS - 1 - pos0 - a.first),
+                        [&](auto tag) {
+            f32x4 s[NQ][SUBS];
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t) {
+            for (int t = 0; t < SUBS; ++t) {
 #pragma unroll
-            for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int dc = 0; dc < DC; ++dc) {
-                const typename Frag<T>::Row kf = row_frag<T, DP>(ks, 16 * t + c, dc, g);
+                for (int dc = 0; dc < DC; ++dc) {
+                    const typename Frag<T>::Row kf = row_frag<T, DP>(ks, 16 * t + c, dc, g);
 #pragma unroll
-                for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
-            }
-        }
-        const TileKind kind = tile_kind(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), h0 == h1, j0 - pos1 - a.first,
-                                        j0 + ROWS - 1 - pos0 - a.first);
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-            score_tile<false>(a, col[x], kind, j0, g, s[x]);
-            float top = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < SUBS; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[x][t][r]);
-            top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); });
-            const float m_new = fmaxf(m_run[x], top);
-            const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-            const float shrink = exp2_hw(m_run[x] - m_ref);
-            m_run[x] = m_new;
-            float sum = 0.0f;
-#pragma unroll
-            for (int t = 0; t < SUBS; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[x][t][r] = exp2_hw(s[x][t][r] - m_ref);
-                    sum += s[x][t][r];
+                    for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
                 }
-            l[x] = l[x] * shrink + sum;
+            }
+            bool more = false;
+            float top[NQ];
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
+            for (int x = 0; x < NQ; ++x) {
+                score_tile<BIASES, decltype(tag)::kind, false>(a, col[x], j0, g, s[x]);
+                top[x] = s[x][0][0];
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top[x] = fmaxf(top[x], s[x][t][r]);
+                top[x] = reduce_rows(top[x], [](float u, float v) { return fmaxf(u, v); });
+                more = more || top[x] > m_run[x] + kSlack;
+            }
+            // The reference is the largest score up to 2^kSlack: sums and outputs are rescaled only where one exceeds it by
+            // more, which after a few tiles is hardly ever.  (Probabilities up to 2^kSlack cost no precision.)
+            if (__ballot(more) != 0) {
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) {
+                    const float m_new = fmaxf(m_run[x], top[x]);
+                    const float shrink = m_new == -INFINITY ? 1.0f : exp2_hw(m_run[x] - m_new);
+                    m_run[x] = m_new;
+                    l[x] *= shrink;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) {
+                const float m_ref = m_run[x] == -INFINITY ? 0.0f : m_run[x];
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        s[x][t][r] = exp2_hw(s[x][t][r] - m_ref);
+                        sum += s[x][t][r];
+                    }
+                l[x] += sum;
+            }
+            mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
+        });
+        if (j0 + ROWS < keys) {
+            T* next = tiles + (turn ^ 1) * 2 * TILE;     // (everyone has left it: the barrier of the last turn)
+            kr.put(next);
+            vr.put(next + TILE);
+            fetch(j0 + 2 * ROWS);
         }
-        mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
+        __syncthreads();
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
@@ -137,15 +164,16 @@ template <class T, int DP, int NQ> int launch_forward_by(AttentionArgs a, hipStr
     const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
     const int64_t blocks = ceil_div(columns, 64 * NQ) * a.kv_heads * a.batch;
     TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
-    const size_t lds = 2 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T) + bias_lds_bytes(a, 64 * NQ);
-    hipLaunchKernelGGL((attention_fwd<T, DP, NQ>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
+    const size_t lds = 4 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T) + bias_lds_bytes(a, 64 * NQ);
+    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_fwd<T, DP, NQ, BIASES>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a));
     return check_launch("ta_nn_attention");
 }
 
 template <class T, int DP> int launch_forward(AttentionArgs a, hipStream_t st) {
     const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
-    // 32 columns to a wave halve the LDS reads per product, which is what 16-bit products wait for; not where that leaves CUs idle
-    if (sizeof(T) == 2 && ceil_div(columns, 128) * a.kv_heads * a.batch >= 512) return launch_forward_by<T, DP, sizeof(T) == 2 ? 2 : 1>(a, st);
+    // 32 columns to a wave halve the LDS reads per product, which is what 16-bit products wait for; not where that leaves CUs idle,
+    // nor for wide heads, whose accumulators then leave room for two waves to a SIMD only
+    if (sizeof(T) == 2 && DP <= 64 && ceil_div(columns, 128) * a.kv_heads * a.batch >= 512) return launch_forward_by<T, DP, sizeof(T) == 2 && DP <= 64 ? 2 : 1>(a, st);
     return launch_forward_by<T, DP, 1>(a, st);
 }
 
