@@ -109,11 +109,40 @@ __device__ __forceinline__ half8 pack8(f32x4 a, f32x4 b, fp16) {
     return half8{static_cast<_Float16>(a.x), static_cast<_Float16>(a.y), static_cast<_Float16>(a.z), static_cast<_Float16>(a.w),
                  static_cast<_Float16>(b.x), static_cast<_Float16>(b.y), static_cast<_Float16>(b.z), static_cast<_Float16>(b.w)};
 }
-// acc[q][dt] += (tile^T)[dim 16 dt + ..][row] * w[q][row][column], over the 64 rows; w: the D registers of the score tiles.
-// 16-bit: the weights are rounded to the tensors' type, as the matrix instruction takes them (an error of half a step per
-// weight, independent from weight to weight, where the result itself is rounded by as much).
+// ---- products that contract over a tile's rows
+// The weights of one column for 16 SUBS rows, as the matrix instructions take them: fp32 as they are; for 16-bit tensors
+// rounded to their type (an error of half a step per weight, independent from weight to weight, where the result itself is
+// rounded by as much).
+template <class T, int SUBS> struct Weights {
+    typename Frag<T>::Row v[SUBS / 2];                   // step s: rows 32 s + 4 g + i and 32 s + 16 + 4 g + i
+    __device__ __forceinline__ void from_tiles(const f32x4 (&w)[SUBS]) {
+#pragma unroll
+        for (int s = 0; s < SUBS / 2; ++s) v[s] = pack8(w[2 * s], w[2 * s + 1], T{});
+    }
+    // from a row of LDS that holds the column's weights by row number
+    __device__ __forceinline__ void from_lds(const T* p, int g) {
+#pragma unroll
+        for (int s = 0; s < SUBS / 2; ++s) {
+            const u16x4 lo = *reinterpret_cast<const u16x4*>(p + 32 * s + 4 * g), hi = *reinterpret_cast<const u16x4*>(p + 32 * s + 16 + 4 * g);
+            v[s] = __builtin_bit_cast(typename Frag<T>::Row, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+template <int SUBS> struct Weights<float, SUBS> {
+    f32x4 v[SUBS];
+    __device__ __forceinline__ void from_tiles(const f32x4 (&w)[SUBS]) {
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) v[t] = w[t];
+    }
+    __device__ __forceinline__ void from_lds(const float* p, int g) {
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) v[t] = *reinterpret_cast<const f32x4*>(p + 16 * t + 4 * g);
+    }
+};
+
+// acc[q][dt] += (tile^T)[dim 16 dt + ..][row] * w[q][row][column], over the rows
 template <int DP, int NQ, int SUBS, class T>
-__device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ][SUBS], f32x4 (&acc)[NQ][DP / 16], int c, int g) {
+__device__ __forceinline__ void mma_transposed(const T* lds, const Weights<T, SUBS> (&w)[NQ], f32x4 (&acc)[NQ][DP / 16], int c, int g) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
@@ -124,15 +153,12 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ
                 for (int dt = 0; dt < DP / 16; ++dt) {
                     const float a = p[16 * dt];
 #pragma unroll
-                    for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(a, w[q][t][r], acc[q][dt]);
+                    for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(a, w[q].v[t][r], acc[q][dt]);
                 }
             }
     } else {
 #pragma unroll
-        for (int s = 0; s < SUBS / 2; ++s) {
-            typename Frag<T>::Row b[NQ];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) b[q] = pack8(w[q][2 * s], w[q][2 * s + 1], T{});
+        for (int s = 0; s < SUBS / 2; ++s)
 #pragma unroll
             for (int dt = 0; dt < DP / 16; ++dt) {
                 const unsigned short* p = reinterpret_cast<const unsigned short*>(lds) + (32 * s + 4 * g + (c >> 2)) * Tile<T, DP>::LD
@@ -140,10 +166,16 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ
                 const u16x4 lo = read_transposed(p), hi = read_transposed(p + 16 * Tile<T, DP>::LD);
                 const u16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(__builtin_bit_cast(typename Frag<T>::Row, a), b[q], acc[q][dt]);
+                for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(__builtin_bit_cast(typename Frag<T>::Row, a), w[q].v[s], acc[q][dt]);
             }
-        }
     }
+}
+template <int DP, int NQ, int SUBS, class T>
+__device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ][SUBS], f32x4 (&acc)[NQ][DP / 16], int c, int g) {
+    Weights<T, SUBS> packed[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) packed[q].from_tiles(w[q]);
+    mma_transposed<DP, NQ, SUBS, T>(lds, packed, acc, c, g);
 }
 
 // ---- bias and mask of a score
@@ -315,6 +347,25 @@ template <class T, int DP> __device__ __forceinline__ void store_column(T* p, co
     }
 }
 
+// The 127 diagonals of the workgroup's 64 x 64 tile of sums (column 16 wave + c: a query): number d + 63 is distance key - query
+// = d.  `tile`: 64 x 65 floats of LDS that nobody uses any more; number 127 is 0.
+__device__ __forceinline__ void store_diagonals(float* tile, const f32x4 (&sum)[4], int wave, int c, int g, float* out) {
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tile[(16 * t + 4 * g + r) * 65 + 16 * wave + c] = sum[t][r];
+    __syncthreads();
+    const int tid = threadIdx.x;
+    if (tid < 128) {
+        const int diagonal = tid - 63;
+        float total = 0.0f;
+        if (tid < 127)
+            for (int i = max(0, -diagonal); i < 64 - max(0, diagonal); ++i) total += tile[(i + diagonal) * 65 + i];
+        out[tid] = total;
+    }
+}
+
 // LDS for the bias values of the heads that `columns` consecutive columns can span; 0, and the kernels read the table from
 // memory, where that is more than 24 KB
 inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns) {
@@ -327,6 +378,20 @@ inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns) {
 }
 
 inline int biases_of(const AttentionArgs& a) { return a.mask_kind || !a.bias_in_lds ? kAny : a.distances ? kByDistance : kByPair; }
+
+// Many short sequences whose pairs are the same in all of them (or in every mask_period-th): attention_window.hip.
+inline bool is_window(const ta_nn_attention_args& a) {
+    return a.m <= 64 && a.n <= 64 && a.dim <= 64 && a.heads == a.kv_heads && !a.key_lengths && !a.query_start;
+}
+// workgroups per head of its backward pass, each with sequences of one mask: enough to fill the CUs twice, as they hold them
+inline int window_periods(const ta_nn_attention_args& a) { return a.mask_kind ? a.mask_period : 1; }
+inline int window_parts(const ta_nn_attention_args& a, int64_t workgroups) {
+    const int64_t classes = window_periods(a), most = ceil_div(a.batch, classes);
+    const int64_t wanted = ceil_div(workgroups, classes * a.heads);
+    return static_cast<int>(wanted < most ? wanted : most);
+}
+constexpr int kWindowWorkgroups = 1024;
+int launch_window(AttentionArgs a, bool backward, hipStream_t st);
 
 int check_attention(const ta_nn_attention_args* args, AttentionArgs& a);
 int64_t workspace_floats(const ta_nn_attention_args& a, bool backward);

@@ -37,19 +37,26 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
     const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
     const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
     const T* op = static_cast<const T*>(a.out) + b * a.o_sb + head * a.o_sh + query * a.o_sm;
+    const int64_t at = (b * a.heads + head) * a.m + query;
     typename Frag<T>::Row q[DC], go[DC];
     float delta = 0.0f;
 #pragma unroll
     for (int dc = 0; dc < DC; ++dc) {
         q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
         go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
-        const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
         const Vec<T> gv = __builtin_bit_cast(Vec<T>, go[dc]);
+        if (sizeof(T) == 2 && a.out32) {
+            const int d = dc * Frag<T>::D + g * Frag<T>::VE;
+            const float* o = a.out32 + at * a.dim + d;
 #pragma unroll
-        for (int i = 0; i < Frag<T>::VE; ++i) delta += get(o, i) * get(gv, i);
+            for (int i = 0; i < Frag<T>::VE; ++i) delta += d + i < a.dim ? o[i] * get(gv, i) : 0.0f;
+        } else {
+            const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
+#pragma unroll
+            for (int i = 0; i < Frag<T>::VE; ++i) delta += get(o, i) * get(gv, i);
+        }
     }
     delta = reduce_rows(delta, Sum{});
-    const int64_t at = (b * a.heads + head) * a.m + query;
     if (valid && g == 0) a.delta[at] = delta;
     const float top = a.stats[2 * at], inv = a.stats[2 * at + 1];
     const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
@@ -298,20 +305,8 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
                     if (j0 + 16 * t + 4 * g + r < a.n) out[j0 + 16 * t + 4 * g + r] = sum[t][r];
         return;
     }
-    __syncthreads();                                     // the tiles are read: their place holds the sums now, [key][query]
-    float* tile = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tile[(16 * t + 4 * g + r) * 65 + 16 * wave + c] = sum[t][r];
-    __syncthreads();
-    if (tid < 128) {
-        const int diagonal = tid - 63;                   // key - query
-        float total = 0.0f;
-        if (tid < 127)
-            for (int i = max(0, -diagonal); i < 64 - max(0, diagonal); ++i) total += tile[(i + diagonal) * 65 + i];
-        a.partial[(((static_cast<int64_t>(chunk) * a.heads + head) * q_tiles + q_tile) * k_tiles + k_tile) * 128 + tid] = total;
-    }
+    store_diagonals(reinterpret_cast<float*>(smem), sum, wave, c, g,
+                    a.partial + (((static_cast<int64_t>(chunk) * a.heads + head) * q_tiles + q_tile) * k_tiles + k_tile) * 128);
 }
 
 __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
@@ -320,18 +315,35 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v)
     else static_cast<fp16*>(p)[i] = from_float<fp16>(v);
 }
 
-// one workgroup for each bucket and head: the chunks' partial sums in a fixed order, in 64 bits
+// Pairs, first: the chunks' sums of every pair, 64 pairs to a workgroup, its four waves a quarter of the chunks each; 64-bit sums,
+// written in two halves over the first chunk's place.  (Reading them bucket by bucket instead touches a line for every value.)
+__global__ __launch_bounds__(256) void attention_pair_sums(AttentionArgs a) {
+    __shared__ double red[4][64];
+    const int64_t pairs = static_cast<int64_t>(a.m) * a.n, tiles = (pairs + 63) / 64;
+    const int head = static_cast<int>(blockIdx.x / tiles), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t pair = blockIdx.x % tiles * 64 + lane;
+    double sum = 0.0;
+    if (pair < pairs) {
+        const float* p = a.partial + head * pairs + pair;
+        const int c0 = static_cast<int>(static_cast<int64_t>(a.chunks) * wave / 4), c1 = static_cast<int>(static_cast<int64_t>(a.chunks) * (wave + 1) / 4);
+#pragma unroll 8
+        for (int chunk = c0; chunk < c1; ++chunk) sum += p[static_cast<int64_t>(chunk) * a.heads * pairs];
+    }
+    red[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && pair < pairs)
+        a.partial[head * pairs + pair] = static_cast<float>(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
+}
+
+// one workgroup for each bucket and head: the partial sums in a fixed order, in 64 bits
 __global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
     __shared__ double red[4];
     const int bucket = static_cast<int>(blockIdx.x) / a.heads, head = static_cast<int>(blockIdx.x) % a.heads;
     double sum = 0.0;
     if (a.distances == 0) {
         const int64_t pairs = static_cast<int64_t>(a.m) * a.n;
-        const int from = a.pair_starts[bucket], count = a.pair_starts[bucket + 1] - from;
-        for (int64_t e = threadIdx.x; e < static_cast<int64_t>(count) * a.chunks; e += 256) {
-            const int64_t chunk = e / count;
-            sum += a.partial[(chunk * a.heads + head) * pairs + a.pair_order[from + e % count]];
-        }
+        const int from = a.pair_starts[bucket], to = a.pair_starts[bucket + 1];
+        for (int e = from + static_cast<int>(threadIdx.x); e < to; e += 256) sum += a.partial[head * pairs + a.pair_order[e]];
     } else {
         const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64;
         const int64_t entries = static_cast<int64_t>(q_tiles) * k_tiles * 128;
@@ -347,6 +359,16 @@ __global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
     if (threadIdx.x == 0) store_as(a.dtable, static_cast<int64_t>(bucket) * a.heads + head, a.table_dtype, static_cast<float>(sum));
 }
 
+int launch_table_sums(const AttentionArgs& a, hipStream_t st) {
+    if (a.distances == 0) {
+        const int64_t blocks = ceil_div(static_cast<int64_t>(a.m) * a.n, 64) * a.heads;
+        TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "%d x %d pairs", a.m, a.n);
+        hipLaunchKernelGGL(attention_pair_sums, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+    }
+    hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
+    return check_launch("ta_nn_attention_backward");
+}
+
 template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) {
     const size_t tiles = 2 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T), table_tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
     const size_t bias = bias_lds_bytes(a, 1);
@@ -359,7 +381,7 @@ template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) 
         const size_t diagonals = 64 * 65 * 4;
         const size_t lds = table_tiles + bias > diagonals ? table_tiles + bias : diagonals;
         TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_table<T, DP, BIASES>), dim3(static_cast<unsigned>(t_blocks)), dim3(256), lds, st, a));
-        hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
+        return launch_table_sums(a, st);
     }
     return check_launch("ta_nn_attention_backward");
 }
@@ -381,5 +403,9 @@ extern "C" int ta_nn_attention_backward(const ta_nn_attention_args* args, void* 
     a.delta = a.workspace;
     a.partial = a.workspace + static_cast<int64_t>(a.batch) * a.heads * a.m;
     hipStream_t st = static_cast<hipStream_t>(stream);
+    if (ta_nn::is_window(a)) {
+        if (int rc = ta_nn::launch_window(a, true, st)) return rc;
+        return a.dtable ? ta_nn::launch_table_sums(a, st) : 0;
+    }
     TA_NN_BY_TYPE_AND_DIM(a.dtype, a.dim, (ta_nn::launch_backward<T, DP>(a, st)));
 }
