@@ -59,6 +59,7 @@ template <class V, class Op> inline V reduce_wave(V v, Op op) {
 }
 inline void forget(u32x4&) {}
 inline void order_memory() {}
+inline void wave_lds_order() { ta_nn_host::wave_sync(); }
 inline float max_nan(float a, float b) { return a != a || b != b ? NAN : a > b ? a : b; }
 inline float exp2_hw(float x) { return x < -126.0f ? 0.0f : exp2f(x); }
 

@@ -92,15 +92,19 @@ def _on_device(t, name):
         raise HipExtensionError("%s is on %s: the HIP path needs tensors on a HIP device (no CPU fallback)" % (name, t.device))
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream       # what torch.cuda.current_stream(dev).cuda_stream is, without the objects
+
+
 def _launch(name, like, *args):
-    fn = getattr(load(), name)
-    dev = like.device
-    if dev.index != torch.cuda.current_device():
+    fn = getattr(_lib or load(), name)
+    dev = like.get_device()
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):                   # the launch needs the tensor's device current in this thread
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     else:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
-    _check(rc, name)
+        rc = fn(*args, _raw_stream(dev))
+    if rc != 0:
+        _check(rc, name)
 
 
 def check_tensor(t, name, like=None, dtypes=None):
@@ -108,7 +112,7 @@ def check_tensor(t, name, like=None, dtypes=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor" % name)
     _on_device(t, name)
-    if like is not None and t.device != like.device:
+    if like is not None and t.get_device() != like.get_device():
         raise ValueError("%s is on %s, not on %s" % (name, t.device, like.device))
     if dtypes is not None and t.dtype not in dtypes:
         raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d).replace("torch.", "") for d in dtypes), t.dtype))

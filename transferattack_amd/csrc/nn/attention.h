@@ -183,7 +183,7 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ
 // The table's values for a block's heads stand in LDS, multiplied already, by bucket (pairs) or by distance; the latter with
 // its ends repeated kPad times, so that a tile that touches the range at all needs no clamping.
 constexpr int kPad = 192;                                // > 64 rows + 128 columns
-__host__ __device__ inline int bias_entries(const AttentionArgs& a) { return a.distances ? a.distances + 2 * kPad : a.buckets; }
+__host__ __device__ inline int bias_entries(const AttentionArgs& a, int pad = kPad) { return a.distances ? a.distances + 2 * pad : a.buckets; }
 
 __device__ __forceinline__ float table_value(const AttentionArgs& a, int entry, int head) {
     const int bucket = a.distances ? static_cast<const int*>(a.index)[entry] : entry;
@@ -191,11 +191,11 @@ __device__ __forceinline__ float table_value(const AttentionArgs& a, int entry, 
 }
 __device__ __forceinline__ int clamp_distance(const AttentionArgs& a, int e) { return e < 0 ? 0 : e >= a.distances ? a.distances - 1 : e; }
 
-__device__ __forceinline__ void stage_bias(const AttentionArgs& a, float* lds, int h0, int count, int threads) {
-    const int entries = bias_entries(a);
+__device__ __forceinline__ void stage_bias(const AttentionArgs& a, float* lds, int h0, int count, int threads, int pad = kPad) {
+    const int entries = bias_entries(a, pad);
     for (int e = threadIdx.x; e < entries * count; e += threads) {
         const int h = e / entries, i = e % entries;
-        lds[e] = table_value(a, a.distances ? clamp_distance(a, i - kPad) : i, h0 + h);
+        lds[e] = table_value(a, a.distances ? clamp_distance(a, i - pad) : i, h0 + h);
     }
 }
 
@@ -275,18 +275,18 @@ template <int BIASES, class Body> __device__ __forceinline__ void by_kind(Kind k
 }
 
 // s (q.k of rows row0 + 16 t + 4 g + r) -> s'; DOWN: rows are queries, whose distance falls as they rise
-template <int BIASES, int KIND, bool DOWN, int SUBS>
+template <int BIASES, int KIND, bool DOWN, int PAD = kPad, int SUBS>
 __device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column& col, int row0, int g, f32x4 (&s)[SUBS]) {
     const float c = a.scale * kLog2e;
     if constexpr (KIND == kConstant) {
         const int at = DOWN ? col.from - row0 : col.from + row0;       // all on the same side of the range
-        const float add = col.bias[kPad + (at < a.distances / 2 ? 0 : a.distances - 1)];
+        const float add = col.bias[PAD + (at < a.distances / 2 ? 0 : a.distances - 1)];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], c, add);
     } else if constexpr (KIND == kNear) {
-        const float* p = col.bias + kPad + (DOWN ? col.from - row0 - 4 * g : col.from + row0 + 4 * g);
+        const float* p = col.bias + PAD + (DOWN ? col.from - row0 - 4 * g : col.from + row0 + 4 * g);
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
@@ -314,12 +314,12 @@ __device__ __forceinline__ void score_tile(const AttentionArgs& a, const Column&
                 int e = bucket[r];
                 if (distances) e = clamp_distance(a, DOWN ? col.from - row - r : col.from + row + r);
                 if constexpr (BIASES != kAny) {
-                    const float f = fmaf(s[t][r], c, col.bias[distances ? e + kPad : e]);
+                    const float f = fmaf(s[t][r], c, col.bias[distances ? e + PAD : e]);
                     s[t][r] = seen ? f : -INFINITY;
                 } else {
                     float f = -INFINITY;
                     if (seen) {
-                        f = fmaf(s[t][r], c, col.bias ? col.bias[distances ? e + kPad : e] : table_value(a, e, col.head));
+                        f = fmaf(s[t][r], c, col.bias ? col.bias[distances ? e + PAD : e] : table_value(a, e, col.head));
                         if (a.mask_kind) f = masked(f, mask_value(a, col.mask + (row + r) * step));
                     }
                     s[t][r] = f;
@@ -368,11 +368,11 @@ __device__ __forceinline__ void store_diagonals(float* tile, const f32x4 (&sum)[
 
 // LDS for the bias values of the heads that `columns` consecutive columns can span; 0, and the kernels read the table from
 // memory, where that is more than 24 KB
-inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns) {
+inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns, int pad = kPad) {
     const int64_t group = a.heads / a.kv_heads;
     int64_t spans = (columns - 1) / a.m + 2;
     if (spans > group) spans = group;
-    const int64_t bytes = spans * bias_entries(a) * 4;
+    const int64_t bytes = spans * bias_entries(a, pad) * 4;
     a.bias_in_lds = bytes <= 24 * 1024;
     return a.bias_in_lds ? static_cast<size_t>(bytes) : 0;
 }
@@ -392,6 +392,19 @@ inline int window_parts(const ta_nn_attention_args& a, int64_t workgroups) {
 }
 constexpr int kWindowWorkgroups = 1024;
 int launch_window(AttentionArgs a, bool backward, hipStream_t st);
+
+// Few queries against many keys -- the next token of every sequence: attention_few.hip.
+inline bool is_few(const ta_nn_attention_args& a) { return static_cast<int64_t>(a.heads / a.kv_heads) * a.m <= 16 && !is_window(a); }
+// Keys of a workgroup.  At least 512, four times what its waves take at once, and no split at all below 1024 keys: joining costs a
+// launch.  Otherwise as many as make some 2048 workgroups, so that sequences of unequal length even out.
+inline int few_chunk(const ta_nn_attention_args& a) {
+    if (a.n <= 1024) return (a.n + 127) / 128 * 128;
+    const int64_t splits = ceil_div(2048, static_cast<int64_t>(a.batch) * a.kv_heads);
+    const int64_t chunk = ceil_div(ceil_div(a.n, splits), 128) * 128;
+    return static_cast<int>(chunk < 512 ? 512 : chunk);
+}
+inline int few_splits(const ta_nn_attention_args& a) { return static_cast<int>(ceil_div(a.n, few_chunk(a))); }
+int launch_few(AttentionArgs a, hipStream_t st);
 
 int check_attention(const ta_nn_attention_args* args, AttentionArgs& a);
 int64_t workspace_floats(const ta_nn_attention_args& a, bool backward);

@@ -12,7 +12,10 @@ static int table_chunks(const ta_nn_attention_args& a) {
 }
 
 int64_t workspace_floats(const ta_nn_attention_args& a, bool backward) {
-    if (!backward) return 0;
+    if (!backward) {
+        const int splits = is_few(a) ? few_splits(a) : 1;
+        return splits == 1 ? 0 : static_cast<int64_t>(a.batch) * a.kv_heads * splits * (32 + 16 * a.dim);
+    }
     int64_t floats = static_cast<int64_t>(a.batch) * a.heads * a.m;
     if (a.dtable) {
         const int64_t per_chunk = a.distances ? ceil_div(a.m, 64) * ceil_div(a.n, 64) * 128 : static_cast<int64_t>(a.m) * a.n;

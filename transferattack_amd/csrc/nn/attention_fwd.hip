@@ -182,7 +182,7 @@ template <class T, int DP> int launch_forward(AttentionArgs a, hipStream_t st) {
 }  // namespace ta_nn
 
 extern "C" int64_t ta_nn_attention_workspace(const ta_nn_attention_args* args, int backward) {
-    if (args == nullptr) return 0;
+    if (args == nullptr || args->kv_heads < 1 || args->batch < 1 || args->m < 1 || args->n < 1) return 0;
     return ta_nn::workspace_floats(*args, backward != 0);
 }
 
@@ -193,5 +193,6 @@ extern "C" int ta_nn_attention(const ta_nn_attention_args* args, void* stream) {
     if (int rc = ta_nn::check_attention(args, a)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (ta_nn::is_window(a)) return ta_nn::launch_window(a, false, st);
+    if (ta_nn::is_few(a)) return ta_nn::launch_few(a, st);
     TA_NN_BY_TYPE_AND_DIM(a.dtype, a.dim, (ta_nn::launch_forward<T, DP>(a, st)));
 }

@@ -48,7 +48,7 @@ __device__ __forceinline__ void window_bias(const AttentionArgs& a, const Share&
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int key = 16 * t + 4 * g + r;
-                if (query < a.m && key < a.n) add[t][r] = masked(add[t][r], mask_value(a, col.mask + key * a.mask_sn));
+                if (add[t][r] != -INFINITY) add[t][r] = masked(add[t][r], mask_value(a, col.mask + key * a.mask_sn));
             }
     }
 }

@@ -76,6 +76,15 @@ __device__ __forceinline__ void order_memory() {
 #endif
 }
 
+// a wave's own LDS writes are seen by its later reads: the hardware does them in order, the compiler has to as well
+__device__ __forceinline__ void wave_lds_order() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#endif
+}
+
 // the larger one, NaN if either is one
 __device__ __forceinline__ float max_nan(float a, float b) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -132,22 +132,27 @@ def _total(row_loss, weight, n, mean, loss, scale):
                 _nn.ptr(loss), _nn.ptr(scale))
 
 
+def _loss(rows, o, save):
+    """-> loss, statistics of the rows and the mean's scale for a backward pass (or None)"""
+    weight, reduction = o[4], o[5]
+    n, dev = rows.shape[0], rows.device
+    row_loss = torch.empty(n, dtype=torch.float32, device=dev)
+    stats = torch.empty((n, STATS), dtype=torch.float32, device=dev) if save else None
+    _nn._launch("ta_nn_distil", rows, *_head(rows, o), 1.0, None, row_loss.data_ptr(), _nn.ptr(stats), None, 0)
+    if reduction == "none":
+        return row_loss, stats, None
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    scale = torch.empty((), dtype=torch.float32, device=dev) if save and weight is not None and reduction == "mean" else None
+    _total(row_loss, weight, n, reduction == "mean", loss, scale)
+    return loss, stats, scale
+
+
 class _Distillation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, o, save):
-        weight, reduction = o[4], o[5]
-        n, dev = rows.shape[0], rows.device
-        row_loss = torch.empty(n, dtype=torch.float32, device=dev)
-        stats = torch.empty((n, STATS), dtype=torch.float32, device=dev) if save else None
-        _nn._launch("ta_nn_distil", rows, *_head(rows, o), 1.0, None, row_loss.data_ptr(), _nn.ptr(stats), None, 0)
-        scale, loss = None, row_loss
-        if reduction != "none":
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            scale = torch.empty((), dtype=torch.float32, device=dev) if weight is not None and reduction == "mean" else None
-            _total(row_loss, weight, n, reduction == "mean", loss, scale)
-        if save:
-            ctx.save_for_backward(rows, stats, scale)
-            ctx.options = o
+    def forward(ctx, rows, o):
+        loss, stats, scale = _loss(rows, o, True)
+        ctx.save_for_backward(rows, stats, scale)
+        ctx.options = o
         return loss
 
     @staticmethod
@@ -161,7 +166,7 @@ class _Distillation(torch.autograd.Function):
         factor = 1.0 / rows.shape[0] if reduction == "mean" and weight is None else 1.0
         _nn._launch("ta_nn_distil_backward", rows, *_head(rows, o), factor, _nn.ptr(scale), upstream.data_ptr(), int(reduction == "none"),
                     stats.data_ptr(), grad.data_ptr(), grad.shape[1])
-        return grad, None, None
+        return grad, None
 
 
 def distillation_loss(logits, answers, weight=None, reduction="mean"):
@@ -175,7 +180,10 @@ def distillation_loss(logits, answers, weight=None, reduction="mean"):
     o = _checked(rows, answers, weight, reduction)
     if rows.shape[0] == 0:
         return rows.float().sum(dim=1) if reduction == "none" else rows.float().sum()
-    loss = _Distillation.apply(rows, o, torch.is_grad_enabled() and rows.requires_grad)
+    if torch.is_grad_enabled() and rows.requires_grad:
+        loss = _Distillation.apply(rows, o)
+    else:
+        loss = _loss(rows, o, False)[0]
     return loss.view(logits.shape[:-1]) if reduction == "none" else loss
 
 

@@ -158,14 +158,6 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
     return o
 
 
-def _strides(args, name, t, prefix, token):
-    setattr(args, name, t.data_ptr())
-    sb, sh, st, _ = t.stride()
-    setattr(args, prefix + "sb", sb)
-    setattr(args, prefix + "sh", sh)
-    setattr(args, prefix + token, st)
-
-
 def _arguments(q, k, v, table, out, stats, o):
     a = _nn.AttentionArgs()
     a.dtype, a.batch, a.heads, a.m, a.dim = _nn.DTYPES[q.dtype], q.shape[0], q.shape[1], q.shape[2], q.shape[3]
@@ -248,12 +240,11 @@ def _token_major(batch, heads, tokens, dim, like):
 
 class _RelativeAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, o, save):
+    def forward(ctx, q, k, v, table, o):
         out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
-        stats, out32 = _forward(q, k, v, table, out, o, save)
-        if save:
-            ctx.save_for_backward(q, k, v, table, out, stats, out32)
-            ctx.options = o
+        stats, out32 = _forward(q, k, v, table, out, o, True)
+        ctx.save_for_backward(q, k, v, table, out, stats, out32)
+        ctx.options = o
         return out
 
     @staticmethod
@@ -264,31 +255,34 @@ class _RelativeAttention(torch.autograd.Function):
         dk = _token_major(k.shape[0], k.shape[1], k.shape[2], k.shape[3], k)
         dv = _token_major(v.shape[0], v.shape[1], v.shape[2], v.shape[3], v)
         dtable = _backward(q, k, v, table, out, stats, out32, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options)
-        return dq, dk, dv, dtable, None, None
+        return dq, dk, dv, dtable, None
+
+
+def _packed_forward(qkv, table, o, save):
+    b, n, _, heads, dim = qkv.shape
+    out = torch.empty((b, n, heads, dim), dtype=qkv.dtype, device=qkv.device)
+    q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
+    return (out,) + _forward(q, k, v, table, out.transpose(1, 2), o, save)
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, table, o, save):
-        b, n, _, heads, dim = qkv.shape
-        out = torch.empty((b, n, heads, dim), dtype=qkv.dtype, device=qkv.device)
-        q, k, v = (qkv.select(2, i).transpose(1, 2) for i in range(3))
-        stats, out32 = _forward(q, k, v, table, out.transpose(1, 2), o, save)
-        if save:
-            ctx.save_for_backward(qkv, table, out, stats, out32)
-            ctx.options = o
-        return out.view(b, n, heads * dim)
+    def forward(ctx, qkv, table, o):
+        out, stats, out32 = _packed_forward(qkv, table, o, True)
+        ctx.save_for_backward(qkv, table, out, stats, out32)
+        ctx.options = o
+        return out.flatten(2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         qkv, table, out, stats, out32 = ctx.saved_tensors
-        q, k, v = (qkv.select(2, i).transpose(1, 2) for i in range(3))
+        q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        dq, dk, dv = (dqkv.select(2, i).transpose(1, 2) for i in range(3))
+        dq, dk, dv = dqkv.permute(2, 0, 3, 1, 4).unbind(0)
         grad = grad.reshape(out.shape).transpose(1, 2)
         dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, out32, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options)
-        return dqkv, dtable, None, None
+        return dqkv, dtable, None
 
 
 def _dense_rows(t, token=2):
@@ -323,7 +317,12 @@ def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=Fa
     save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)
     if save and table.requires_grad and o.start_tensor is not None and buckets.distances:
         raise ValueError("the table's gradient needs one query_start for all sequences (an int)")
-    return _RelativeAttention.apply(_dense_rows(q), _dense_rows(k), _dense_rows(v), table.contiguous(), o, save)
+    q, k, v, table = _dense_rows(q), _dense_rows(k), _dense_rows(v), table.contiguous()
+    if save:
+        return _RelativeAttention.apply(q, k, v, table, o)
+    out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
+    _forward(q, k, v, table, out, o, False)
+    return out
 
 
 def relative_attention_packed(qkv, table, buckets, scale=None, mask=None, causal=False, key_lengths=None):
@@ -335,4 +334,5 @@ def relative_attention_packed(qkv, table, buckets, scale=None, mask=None, causal
     q = qkv.detach().select(2, 0).transpose(1, 2)
     o = _options(q, q, table, buckets, scale, mask, causal, key_lengths, 0)
     save = torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad)
-    return _PackedAttention.apply(_dense_rows(qkv, 1), table.contiguous(), o, save)
+    qkv, table = _dense_rows(qkv, 1), table.contiguous()
+    return _PackedAttention.apply(qkv, table, o) if save else _packed_forward(qkv, table, o, False)[0].flatten(2)
