@@ -69,9 +69,6 @@ typedef struct ta_nn_attention_args {
     int64_t o_sb, o_sh, o_sm;
     float* stats;                                /* [batch][heads][m][2]: maximum of the scores and 1 / sum of the exponentials,
                                                     for a backward pass; or NULL */
-    float* out32;                                /* [batch][heads][m][dim]: out unrounded, or NULL.  A 16-bit forward pass writes it, the
-                                                    backward pass reads it: the table's gradient is a sum of differences that a
-                                                    rounded output disturbs.  Not used where ta_nn_attention_is_window() */
     float* workspace;                            /* ta_nn_attention_workspace() floats, or NULL where that is 0 */
     /* backward: */
     const void* grad;                            /* of out; out and stats are the forward pass's */
@@ -84,8 +81,6 @@ typedef struct ta_nn_attention_args {
 } ta_nn_attention_args;
 
 int64_t ta_nn_attention_workspace(const ta_nn_attention_args* args, int backward);
-/* whether a call is one of many short sequences (m, n, dim <= 64, no shared heads, no lengths or positions by sequence) */
-int ta_nn_attention_is_window(const ta_nn_attention_args* args);
 int ta_nn_attention(const ta_nn_attention_args* args, void* stream);
 int ta_nn_attention_backward(const ta_nn_attention_args* args, void* stream);
 

@@ -30,7 +30,7 @@ class AttentionArgs(ctypes.Structure):
                 + [(n, _i64) for n in ("mask_sb", "mask_sh", "mask_sm", "mask_sn")]
                 + [("key_lengths", _vp), ("query_start", _vp), ("start", _int), ("causal", _int), ("out", _vp)]
                 + [(n, _i64) for n in ("o_sb", "o_sh", "o_sm")]
-                + [("stats", _vp), ("out32", _vp), ("workspace", _vp), ("grad", _vp)]
+                + [("stats", _vp), ("workspace", _vp), ("grad", _vp)]
                 + [(n, _i64) for n in ("g_sb", "g_sh", "g_sm")]
                 + [(n, _vp) for n in ("dq", "dk", "dv")]
                 + [(n, _i64) for n in ("dq_sb", "dq_sh", "dq_sm", "dk_sb", "dk_sh", "dk_sn", "dv_sb", "dv_sh", "dv_sn")]
@@ -44,7 +44,6 @@ SIGNATURES = {
     "ta_nn_abi_version": (_int, []),
     "ta_nn_last_error": (ctypes.c_char_p, []),
     "ta_nn_attention_workspace": (_i64, [_args_p, _int]),
-    "ta_nn_attention_is_window": (_int, [_args_p]),
     "ta_nn_attention": (_int, [_args_p, _vp]),
     "ta_nn_attention_backward": (_int, [_args_p, _vp]),
     "ta_nn_top_logits": (_int, [_vp, _int, _i64, _i64, _int, _int, _f32, _vp, _vp, _vp, _vp]),

@@ -45,23 +45,18 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
         q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
         go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
         const Vec<T> gv = __builtin_bit_cast(Vec<T>, go[dc]);
-        if (sizeof(T) == 2 && a.out32) {
-            const int d = dc * Frag<T>::D + g * Frag<T>::VE;
-            const float* o = a.out32 + at * a.dim + d;
+        const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
 #pragma unroll
-            for (int i = 0; i < Frag<T>::VE; ++i) delta += d + i < a.dim ? o[i] * get(gv, i) : 0.0f;
-        } else {
-            const Vec<T> o = __builtin_bit_cast(Vec<T>, row_frag_global<T>(op, a.dim, dc, g, valid));
-#pragma unroll
-            for (int i = 0; i < Frag<T>::VE; ++i) delta += get(o, i) * get(gv, i);
-        }
+        for (int i = 0; i < Frag<T>::VE; ++i) delta += get(o, i) * get(gv, i);
     }
     delta = reduce_rows(delta, Sum{});
-    if (valid && g == 0) a.delta[at] = delta;
     const float top = a.stats[2 * at], inv = a.stats[2 * at + 1];
     const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
     const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
 
+    // delta for this kernel is out . grad.  For 16-bit tensors out is rounded, and so were the probabilities it was made with; for
+    // the table, whose gradient is a sum of differences that nearly cancel, and for the keys it is taken anew: sum_j p_ij dp_ij.
+    float exact = 0.0f;
     f32x4 dq[1][DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -97,12 +92,15 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = exp2_hw(s[t][r] - top) * inv;
-                ds[0][t][r] = p == 0.0f ? 0.0f : p * (ds[0][t][r] - delta);       // a masked value may be anything
+                const float p = exp2_hw(s[t][r] - top) * inv, dp = p == 0.0f ? 0.0f : ds[0][t][r];      // a masked value may be anything
+                ds[0][t][r] = p * (dp - delta);
+                exact += p * dp;
             }
         mma_transposed<DP, 1, SUBS>(ks, ds, dq, c, g);
         });
     }
+    exact = reduce_rows(exact, Sum{});
+    if (valid && g == 0) a.delta[at] = exact;
     if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
 }
 

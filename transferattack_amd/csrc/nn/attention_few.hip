@@ -166,7 +166,6 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
             f *= sum == 0.0f ? 0.0f : 1.0f / sum;
             const int h = hk * group + x / a.m, i = x % a.m;
             static_cast<T*>(a.out)[b * a.o_sb + h * a.o_sh + i * a.o_sm + d] = from_float<T>(f);
-            if (sizeof(T) == 2 && a.out32) a.out32[((b * a.heads + h) * a.m + i) * a.dim + d] = f;
         }
     }
 }
@@ -212,10 +211,6 @@ template <class T> __global__ __launch_bounds__(64) void attention_join(Attentio
     const int64_t row = (b * a.heads + head) * a.m + query;
     if (lane < a.dim) out[d0] = from_float<T>(f0 * inv);
     if (lane + 64 < a.dim) out[d1] = from_float<T>(f1 * inv);
-    if (sizeof(T) == 2 && a.out32) {
-        if (lane < a.dim) a.out32[row * a.dim + d0] = f0 * inv;
-        if (lane + 64 < a.dim) a.out32[row * a.dim + d1] = f1 * inv;
-    }
     if (a.stats && lane == 0) {
         a.stats[2 * row] = m_ref;
         a.stats[2 * row + 1] = inv;

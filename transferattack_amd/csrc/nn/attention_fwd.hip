@@ -153,7 +153,6 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
         T* p = static_cast<T*>(a.out) + b * a.o_sb + col[x].head * a.o_sh + query[x] * a.o_sm;
         store_column<T, DP>(p, o[x], inv, a.dim, g);
         const int64_t row = (b * a.heads + col[x].head) * a.m + query[x];
-        if (sizeof(T) == 2 && a.out32) store_column<float, DP>(a.out32 + row * a.dim, o[x], inv, a.dim, g);
         if (a.stats && g == 0) {
             float* st = a.stats + 2 * row;
             st[0] = m_run[x] == -INFINITY ? 0.0f : m_run[x];
@@ -185,8 +184,6 @@ extern "C" int64_t ta_nn_attention_workspace(const ta_nn_attention_args* args, i
     if (args == nullptr || args->kv_heads < 1 || args->batch < 1 || args->m < 1 || args->n < 1) return 0;
     return ta_nn::workspace_floats(*args, backward != 0);
 }
-
-extern "C" int ta_nn_attention_is_window(const ta_nn_attention_args* args) { return args != nullptr && ta_nn::is_window(*args) ? 1 : 0; }
 
 extern "C" int ta_nn_attention(const ta_nn_attention_args* args, void* stream) {
     ta_nn::AttentionArgs a{};

@@ -192,25 +192,21 @@ def _workspace(a, like, backward):
 
 
 def _forward(q, k, v, table, out, o, save):
-    """-> (statistics, unrounded output) for a backward pass, or (None, None)"""
+    """-> statistics for a backward pass, or None"""
     stats = torch.empty(q.shape[:3] + (2,), dtype=torch.float32, device=q.device) if save else None
-    out32 = None
     if out.numel() == 0:
-        return stats, out32
+        return stats
     if k.shape[2] == 0:
         out.zero_()
-        return stats, out32
+        return stats
     a = _arguments(q, k, v, table, out, stats, o)
-    if save and table.requires_grad and q.dtype != torch.float32 and not _nn.load().ta_nn_attention_is_window(a):
-        out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-        a.out32 = out32.data_ptr()
     ws = _workspace(a, q, False)                         # kept alive until the launches are enqueued
     _nn._launch("ta_nn_attention", q, a)
     del ws
-    return stats, out32
+    return stats
 
 
-def _backward(q, k, v, table, out, stats, out32, grad, dq, dk, dv, table_grad, o):
+def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
     dtable = torch.zeros_like(table) if table_grad else None
     if out.numel() == 0 or k.shape[2] == 0:
         for t in (dq, dk, dv):
@@ -218,7 +214,7 @@ def _backward(q, k, v, table, out, stats, out32, grad, dq, dk, dv, table_grad, o
         return dtable
     grad = _dense_rows(grad)
     a = _arguments(q, k, v, table, out, stats, o)
-    a.out32, a.grad = _nn.ptr(out32), grad.data_ptr()
+    a.grad = grad.data_ptr()
     a.g_sb, a.g_sh, a.g_sm, _ = grad.stride()
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     a.dq_sb, a.dq_sh, a.dq_sm, _ = dq.stride()
@@ -242,19 +238,19 @@ class _RelativeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, o):
         out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
-        stats, out32 = _forward(q, k, v, table, out, o, True)
-        ctx.save_for_backward(q, k, v, table, out, stats, out32)
+        stats = _forward(q, k, v, table, out, o, True)
+        ctx.save_for_backward(q, k, v, table, out, stats)
         ctx.options = o
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, table, out, stats, out32 = ctx.saved_tensors
+        q, k, v, table, out, stats = ctx.saved_tensors
         dq = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
         dk = _token_major(k.shape[0], k.shape[1], k.shape[2], k.shape[3], k)
         dv = _token_major(v.shape[0], v.shape[1], v.shape[2], v.shape[3], v)
-        dtable = _backward(q, k, v, table, out, stats, out32, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options)
+        dtable = _backward(q, k, v, table, out, stats, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options)
         return dq, dk, dv, dtable, None
 
 
@@ -262,26 +258,26 @@ def _packed_forward(qkv, table, o, save):
     b, n, _, heads, dim = qkv.shape
     out = torch.empty((b, n, heads, dim), dtype=qkv.dtype, device=qkv.device)
     q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
-    return (out,) + _forward(q, k, v, table, out.transpose(1, 2), o, save)
+    return out, _forward(q, k, v, table, out.transpose(1, 2), o, save)
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, o):
-        out, stats, out32 = _packed_forward(qkv, table, o, True)
-        ctx.save_for_backward(qkv, table, out, stats, out32)
+        out, stats = _packed_forward(qkv, table, o, True)
+        ctx.save_for_backward(qkv, table, out, stats)
         ctx.options = o
         return out.flatten(2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        qkv, table, out, stats, out32 = ctx.saved_tensors
+        qkv, table, out, stats = ctx.saved_tensors
         q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = dqkv.permute(2, 0, 3, 1, 4).unbind(0)
         grad = grad.reshape(out.shape).transpose(1, 2)
-        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, out32, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options)
+        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options)
         return dqkv, dtable, None
 
 
