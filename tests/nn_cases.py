@@ -251,3 +251,123 @@ def check_distil(rows, classes, top, dtype, device, temperature=2.0, rest=True, 
         nn_oracle.close("loss of the one-pass form", both[0], (loss.sum() * by, loss_bound.sum() * by + 2 * nn_oracle.U * loss.abs().sum() * by + 1e-30))
         nn_oracle.close("gradient of the one-pass form", both[1], (grad, grad_bound))
     return got, dx
+
+
+def _twice(s, v, c, r, w):
+    c[:, 1] = c[:, 0]                                    # a class given twice counts with both masses
+    return s, v, c, r, w
+
+
+def _none(s, v, c, r, w):
+    c[:, 1:] = -1
+    c[0] = -1                                            # a row without any answer
+    return s, v, c, r, w
+
+
+def _minus_infinity(s, v, c, r, w):
+    s[:, 0] = -torch.inf                                 # the student rules out a class that was not answered
+    c[c == 0] = 1
+    v[0, -1] = -torch.inf                                # the teacher rules out one it answers
+    return s, v, c, r, w
+
+
+def _nothing_counts(s, v, c, r, w):
+    return s, v, c, r, torch.zeros_like(w)
+
+
+DISTIL_ODD = {
+    "twice": (dict(rows=3, classes=50, top=4, rest=True, change=_twice)),
+    "twice without rest": (dict(rows=3, classes=50, top=4, rest=False, change=_twice)),
+    "no answers": (dict(rows=3, classes=50, top=4, rest=True, change=_none)),
+    "no answers without rest": (dict(rows=3, classes=50, top=4, rest=False, change=_none)),
+    "minus infinity": (dict(rows=4, classes=60, top=5, rest=True, change=_minus_infinity)),
+    "nothing counts": (dict(rows=4, classes=60, top=5, rest=True, weighted=True, change=_nothing_counts)),
+    "nothing counts, sum": (dict(rows=4, classes=60, top=5, rest=True, weighted=True, change=_nothing_counts, reduction="sum")),
+}
+
+
+def check_distil_odd(name, device, dtype=F32):
+    options = dict(DISTIL_ODD[name])
+    rows, classes, top = (options.pop(k) for k in ("rows", "classes", "top"))
+    check_distil(rows, classes, top, dtype, device, **options)
+
+
+def check_class_out_of_range(device):
+    """such a row's loss and gradient are NaN, its neighbours are not touched"""
+    student, values, order, left, _ = distil_inputs(3, 40, 4, F32)
+    order[1, 2] = 40
+    answers = TopLogits(values.to(device), order.to(device), left.to(device), 2.0)
+    x = student.to(device).requires_grad_(True)
+    loss = distillation_loss(x, answers, reduction="none")
+    (dx,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert torch.equal(loss.isnan().cpu(), torch.tensor([False, True, False]))
+    assert not dx[0].isnan().any() and dx[1].isnan().all() and not dx[2].isnan().any()
+    got = distillation_loss_and_grad(x, answers)[1]
+    assert got[1].isnan().all() and not got[0].isnan().any()
+
+
+def check_differences(device):
+    """the kernels' gradients against differences of the 64-bit definitions along a random direction: (f(x + h d) - f(x - h d)) / 2h
+    is off by h^2 / 6 times a third derivative (of order 10 here) and 2^-52 |f| / h: below 1e-8 for h = 1e-5"""
+    h = 1e-5
+    c = case(m=11, n=13, heads=4, kv=2, pairs=False, causal=True, seed=3)
+    x, plan, options, want = make_attention(c, device)
+    leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v", "table")]
+    grads = torch.autograd.grad(relative_attention(*leaves, plan, **options), leaves, x["grad"])
+    gen = torch.Generator().manual_seed(5)
+    key, query = torch.arange(13), torch.arange(11)
+    allowed = (key[None] <= query[:, None]).expand(2, 4, 11, 13)
+    line = plan.source.cpu()
+    bucket = line[(key[None] - query[:, None] + 6).clamp(0, 13)][None]
+    base = [t.detach().cpu().double() for t in leaves]
+    for i, name in enumerate(("dq", "dk", "dv", "dtable")):
+        d = torch.randn(base[i].shape, generator=gen).double()
+        f = []
+        for sign in (1, -1):
+            moved = [b + sign * h * d if j == i else b for j, b in enumerate(base)]
+            out = nn_oracle.attention(*moved, bucket, 32 ** -0.5, allowed, None, None, F32)["out"][0]
+            f.append(float((out * x["grad"].cpu().double()).sum()))
+        along = float((grads[i].detach().cpu().double() * d).sum())
+        assert abs(along - (f[0] - f[1]) / (2 * h)) <= float((want[name][1] * d.abs()).sum()) + 1e-7, name
+    student, values, order, left, _ = distil_inputs(4, 70, 5, F32, seed=9)
+    answers = TopLogits(values.to(device), order.to(device), left.to(device), 2.0)
+    (loss, _), (_, bound) = nn_oracle.distillation(student, values, order, left, 2.0, None, F32, torch.full((4,), 0.25))
+    grad = distillation_loss_and_grad(student.to(device), answers)[1].cpu().double()
+    d = torch.randn(student.shape, generator=gen).double()
+    f = [nn_oracle.distillation(student.double() + s * h * d, values, order, left, 2.0, None, F32, torch.full((4,), 0.25))[0][0].mean() for s in (1, -1)]
+    assert abs(float((grad * d).sum()) - float(f[0] - f[1]) / (2 * h)) <= float((bound * d.abs()).sum()) + 1e-7
+
+
+def check_broadcast_inputs(device):
+    """inputs expanded over the batch (stride 0): read as they are, their gradients summed by autograd"""
+    gen = torch.Generator().manual_seed(1)
+    q, k, grad = (torch.randn(s, generator=gen).to(device) for s in ((3, 2, 6, 32), (1, 2, 9, 32), (3, 2, 6, 32)))
+    v, table = torch.randn((1, 2, 9, 32), generator=gen).to(device), torch.randn((5, 2), generator=gen).to(device)
+    plan = RelativeBuckets.from_index(torch.randint(0, 5, (6, 9), generator=gen).to(device))
+    results = []
+    for copy in (False, True):
+        kk, vv = k.clone().requires_grad_(True), v.clone().requires_grad_(True)
+        ke, ve = kk.expand(3, -1, -1, -1), vv.expand(3, -1, -1, -1)
+        out = relative_attention(q, ke.contiguous() if copy else ke, ve.contiguous() if copy else ve, table, plan)
+        results.append((out,) + torch.autograd.grad(out, (kk, vv), grad))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+def check_empty(device):
+    """no sequence, no query, no key, no row"""
+    table = torch.zeros((3, 2), device=device, requires_grad=True)
+    plan = RelativeBuckets.by_distance(torch.tensor([0, 1, 2]).to(device), -1)
+    for batch, m, n in ((0, 4, 5), (2, 0, 5), (2, 4, 0)):
+        q = torch.randn(batch, 2, m, 16, device=device, requires_grad=True)
+        k, v = (torch.randn(batch, 2, n, 16, device=device, requires_grad=True) for _ in range(2))
+        out = relative_attention(q, k, v, table, plan)
+        assert out.shape == q.shape and not out.any()
+        for g, t in zip(torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out)), (q, k, v, table)):
+            assert g.shape == t.shape and not g.any()
+    assert len(top_logits(torch.empty(0, 9, device=device), 3)) == 0
+    x = torch.empty(0, 9, device=device, requires_grad=True)
+    answers = top_logits(x, 3)
+    loss = distillation_loss(x, answers)
+    assert float(loss.detach()) == 0.0 and torch.autograd.grad(loss, x)[0].shape == x.shape
+    assert float(distillation_loss_and_grad(x, answers)[0]) == 0.0

@@ -53,24 +53,31 @@ def attention(q, k, v, table, bucket, scale, allowed, added, grad, dtype):
     dp = g @ vv.transpose(-2, -1)
     dp_err = (dim + 4) * U * (g.abs() @ vv.abs().transpose(-2, -1))
     delta = (out * g).sum(-1, keepdim=True)
-    delta_err = (got["out"][1] * g.abs()).sum(-1, keepdim=True) + (dim + 4) * U * (out * g).abs().sum(-1, keepdim=True)
+    # dq's kernel takes delta from the rounded output; for the keys and the table it is sum_j p dp in 32 bits
+    delta_q = (got["out"][1] * g.abs()).sum(-1, keepdim=True) + (dim + 4) * U * (out * g).abs().sum(-1, keepdim=True)
+    delta_k = ((p * (rel + n * U) + tiny) * dp.abs() + p * dp_err).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    ds_err = (p * rel + tiny) * (dp - delta).abs() + p * (1 + rel) * (dp_err + delta_err) + 2 * U * p * (dp.abs() + delta.abs())
-    pe, dse = p * (rel + t16 + m * group * U) + tiny, ds_err + (t16 + (m * group + n) * U) * ds.abs()
+
+    def ds_err(delta_err):
+        return (p * rel + tiny) * (dp - delta).abs() + p * (1 + rel) * (dp_err + delta_err) + 2 * U * p * (dp.abs() + delta.abs())
+
+    pe = p * (rel + t16 + m * group * U) + tiny
+    dse_q = ds_err(delta_q) + (t16 + n * U) * ds.abs()
+    dse_k = ds_err(delta_k) + (t16 + m * group * U) * ds.abs()
 
     def shared(x):
         return x.view(batch, kv, group, n, dim).sum(2)
 
     dq, dk, dv = ds @ kk * scale, shared(ds.transpose(-2, -1) @ q) * scale, shared(p.transpose(-2, -1) @ g)
     a = abs(scale)
-    got["dq"] = (dq, dse @ kk.abs() * a + (t + 2 * U) * dq.abs() + 1e-30)
-    got["dk"] = (dk, shared(dse.transpose(-2, -1) @ q.abs()) * a + (t + 2 * U) * dk.abs() + 1e-30)
+    got["dq"] = (dq, dse_q @ kk.abs() * a + (t + 2 * U) * dq.abs() + 1e-30)
+    got["dk"] = (dk, shared(dse_k.transpose(-2, -1) @ q.abs()) * a + (t + 2 * U) * dk.abs() + 1e-30)
     got["dv"] = (dv, shared(pe.transpose(-2, -1) @ g.abs()) + t * dv.abs() + 1e-30)
     flat = bucket.expand(batch, m, n).reshape(-1)
     dtable = torch.zeros_like(table).index_add_(0, flat, ds.movedim(1, -1).reshape(-1, heads))
-    err = torch.zeros_like(table).index_add_(0, flat, ds_err.movedim(1, -1).reshape(-1, heads))
+    err = torch.zeros_like(table).index_add_(0, flat, ds_err(delta_k).movedim(1, -1).reshape(-1, heads))
     mass = torch.zeros_like(table).index_add_(0, flat, ds.abs().movedim(1, -1).reshape(-1, heads))
-    got["dtable"] = (dtable, err + (batch + 64) * U * mass, )
+    got["dtable"] = (dtable, err + (batch + 64) * U * mass)
     return got
 
 

@@ -59,3 +59,214 @@ def test_top_logits(rows, classes, top, dtype, kind):
     (7, 21841, 17, F32, dict(weighted=True)), (6, 32768, 32, BF16, dict(stride=1)), (3, 65537, 1024, F16, {}), (2, 300001, 5, F32, {})])
 def test_distillation(rows, classes, top, dtype, options):
     cases.check_distil(rows, classes, top, dtype, DEV, **options)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("name", sorted(cases.DISTIL_ODD))
+def test_distillation_odd(name, dtype):
+    cases.check_distil_odd(name, DEV, dtype)
+
+
+def test_class_out_of_range():
+    cases.check_class_out_of_range(DEV)
+
+
+def test_gradients_against_differences():
+    cases.check_differences(DEV)
+
+
+def test_broadcast_inputs():
+    cases.check_broadcast_inputs(DEV)
+
+
+def test_empty():
+    cases.check_empty(DEV)
+
+
+# forward and backward of every kernel family: windows, tiles by pair and by distance, few queries with and without a split
+FAMILIES = {
+    "windows": case(m=49, batch=40, heads=3, dim=32, mask="windows", buckets=169),
+    "pairs": case(m=100, batch=2, heads=2, dim=64, buckets=50, dtype=BF16),
+    "distances": case(m=200, batch=2, heads=4, kv=2, dim=64, pairs=False, causal=True, dtype=F16),
+    "masked": case(m=90, n=110, batch=2, heads=2, dim=32, mask="bool"),
+    "few": case(m=2, n=700, batch=2, heads=4, kv=1, dim=64, pairs=False, start=690),
+    "few, split": case(m=1, n=3000, batch=2, heads=4, kv=2, dim=64, pairs=False, start=2999, dtype=BF16),
+}
+
+
+def _step(x, plan, options):
+    from transferattack_amd.relative import relative_attention
+    leaves = [x[n].detach().requires_grad_(True) for n in ("q", "k", "v", "table")]
+    out = relative_attention(*leaves, plan, **options)
+    return (out.detach(),) + torch.autograd.grad(out, leaves, x["grad"])
+
+
+@pytest.mark.parametrize("name", sorted(FAMILIES))
+def test_attention_in_a_graph(name):
+    """captured forward + backward, replayed between eager work on new inputs: the eager bits every time (the kernels add in a fixed
+    order), the workspaces of two graphs apart"""
+    c = FAMILIES[name]
+    x, plan, options, want = cases.make_attention(c, DEV)
+    static = {n: t.clone() for n, t in x.items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(static, plan, options)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outputs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outputs.append(_step(static, plan, options))
+        graphs.append(g)
+    for turn in range(3):
+        other = cases.make_attention(dict(c, seed=turn + 10), DEV)[0]
+        eager = _step(other, plan, options)
+        for n, t in other.items():
+            static[n].copy_(t)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for captured in outputs:
+            assert all(torch.equal(a, b) for a, b in zip(captured, eager)), (name, turn)
+
+
+def test_distillation_in_a_graph():
+    student, values, order, left, weight = (t.to(DEV) for t in cases.distil_inputs(16, 3000, 6, F32, weighted=True))
+    from transferattack_amd.distill import TopLogits, distillation_loss, distillation_loss_and_grad, top_logits
+
+    def step(x):
+        x = x.detach().requires_grad_(True)
+        loss = distillation_loss(x, TopLogits(values, order, left, 2.0), weight=weight)
+        (dx,) = torch.autograd.grad(loss, x)
+        answers = top_logits(x, 6, temperature=2.0)
+        return (loss.detach(), dx, answers.values, answers.classes, answers.rest) + distillation_loss_and_grad(x, TopLogits(values, order, left, 2.0))
+
+    static = student.clone()
+    step(static)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step(static)
+    for turn in range(3):
+        x = student + turn
+        eager = step(x)
+        static.copy_(x)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.nan_to_num(1e9), b.nan_to_num(1e9)) for a, b in zip(captured, eager)), turn
+
+
+def test_two_streams_at_once():
+    """calls of every family on two streams, several in flight on each, give the bits they give alone"""
+    made = [(name, cases.make_attention(dict(FAMILIES[name], seed=s), DEV)) for s in (0, 1) for name in sorted(FAMILIES)]
+    alone = [_step(x, plan, options) for _, (x, plan, options, _) in made]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    results = [None] * len(made)
+    for turn in range(2):
+        for i, (_, (x, plan, options, _)) in enumerate(made):
+            with torch.cuda.stream(streams[i % 2]):
+                results[i] = _step(x, plan, options)
+        torch.cuda.synchronize()
+        for a, b, (name, _) in zip(results, alone, made):
+            assert all(torch.equal(u, v) for u, v in zip(a, b)), (name, turn)
+
+
+def test_long_cache_behind_2_31():
+    """a cache whose last sequence lies more than 2^31 elements behind the first, queries over it"""
+    from transferattack_amd.relative import RelativeBuckets, relative_attention
+    n, dim, batch = 70000, 128, 3
+    room = torch.zeros((batch, 120 * n, dim), dtype=BF16, device=DEV)           # 3.2e9 elements, 6.5 GB
+    k, v = room[:, None, :n], room[:, None, n:2 * n]
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    k.copy_(torch.randn(k.shape, generator=gen, device=DEV))
+    v.copy_(torch.randn(v.shape, generator=gen, device=DEV))
+    q = torch.randn((batch, 4, 1, dim), generator=gen, device=DEV).to(BF16)
+    table = torch.randn((32, 4), generator=gen, device=DEV)
+    plan = RelativeBuckets.logarithmic(32, 128, bidirectional=False, device=DEV)
+    got = relative_attention(q, k, v, table, plan, query_start=n - 1)
+    index = plan.source.cpu().long()[(torch.arange(n) - (n - 1)).clamp(-128, 128) + 128][None, None]
+    for b in (0, 2):
+        want = nn_oracle.attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], table, index, dim ** -0.5, None, None, None, BF16)
+        nn_oracle.close("out", got[b:b + 1], want["out"])
+
+
+def _small_swin(seed):
+    from transferattack_amd.backbones.timm_victims import SwinTransformer
+    torch.manual_seed(seed)
+    net = SwinTransformer(img=56, depths=(2, 2), heads=(3, 6), num_classes=40).eval()
+    for p in net.parameters():
+        if p.dim() > 1:
+            torch.nn.init.normal_(p, std=p.shape[-1] ** -0.5 if p.shape[-1] > 6 else 0.5)
+    return net
+
+
+def test_window_transformer(monkeypatch):
+    """the surrogate's attention on the kernels: logits, input gradient and the bias tables' gradients against the module in 64
+    bits.  Both forms make the same number of fp32 roundings, in another order: the kernels' may be off by four times the module
+    path's own error (whose size is what a rounding's is worth in this network) at most."""
+    x = torch.randn(3, 3, 56, 56, generator=torch.Generator().manual_seed(2))
+    up = torch.randn(3, 40, generator=torch.Generator().manual_seed(3))
+    results = {}
+    for name, dtype, dev, flag in (("truth", torch.float64, "cpu", "0"), ("module", F32, DEV, "0"), ("kernels", F32, DEV, "1")):
+        monkeypatch.setenv("TA_RELATIVE_ATTENTION", flag)
+        net = _small_swin(0).to(dev, dtype)
+        xx = x.to(dev, dtype).requires_grad_(True)
+        tables = [p for n, p in net.named_parameters() if n.endswith("bias_table")]
+        logits = net(xx)
+        results[name] = [t.detach().cpu().double() for t in (logits,) + torch.autograd.grad(logits, [xx] + tables, up.to(dev, dtype))]
+        assert len(results[name]) == 6
+    for truth, module, kernels in zip(*(results[n] for n in ("truth", "module", "kernels"))):
+        own = (module - truth).norm()
+        assert (kernels - truth).norm() <= 4 * own + 1e-7 * truth.norm(), ((kernels - truth).norm(), own)
+
+
+def test_surrogate_learns_from_answers(monkeypatch):
+    """the operators together, as adapting a surrogate to a victim uses them: the victim's answers, the surrogate's forward pass,
+    the loss against the answers, all gradients -- against the same in 64 bits"""
+    from transferattack_amd.distill import distillation_loss, top_logits
+    x = torch.randn(6, 3, 56, 56, generator=torch.Generator().manual_seed(4))
+    monkeypatch.setenv("TA_RELATIVE_ATTENTION", "1")
+    teacher, student = _small_swin(1).to(DEV), _small_swin(0).to(DEV)
+    with torch.no_grad():
+        answers = top_logits(teacher(x.to(DEV)), 5, temperature=2.0)
+    logits = student(x.to(DEV))
+    loss = distillation_loss(logits, answers)
+    parameters = dict(student.named_parameters())
+    grads = dict(zip(parameters, torch.autograd.grad(loss, list(parameters.values()))))
+    reference = _small_swin(0).double()
+    z = reference(x.double()) / 2.0
+    c = answers.classes.cpu()
+    log_q = torch.log_softmax(z, -1)
+    others = torch.ones_like(z, dtype=torch.bool).scatter_(1, c, False)
+    log_q = torch.cat([log_q.gather(1, c), log_q.masked_fill(~others, -torch.inf).logsumexp(-1, keepdim=True)], 1)
+    log_p = torch.log_softmax(torch.cat([answers.values.cpu().double() / 2.0, answers.rest.cpu().double()[:, None]], 1), -1)
+    want = 4.0 * (log_p.exp() * (log_p - log_q)).sum(-1).mean()
+    assert abs(float(loss.detach()) - float(want)) <= 1e-4 * float(want.detach())
+    truth = dict(zip(parameters, torch.autograd.grad(want, [dict(reference.named_parameters())[n] for n in parameters])))
+    # fp32 through eight blocks' forward and backward: some 10^3 roundings of 2^-24 in a row, 1e-4
+    for name in parameters:
+        assert (grads[name].cpu().double() - truth[name]).norm() <= 1e-4 * truth[name].norm() + 1e-9, name
+
+
+def test_attack_on_answers():
+    """an attack with loss='distillation': the first gradient is that of the loss in the image, the run ends in the ball"""
+    import transferattack_amd as ta
+    from transferattack_amd.distill import distillation_loss, top_logits
+    atk = ta.load_attack_class("mifgsm")(model_name="toy_cnn", epoch=3, loss="distillation")
+    x = torch.randint(0, 256, (4, 3, 224, 224), generator=torch.Generator().manual_seed(0)).float() / 255
+    victim = ta.load_attack_class("mifgsm")(model_name="toy_cnn").model
+    with torch.no_grad():
+        for p in victim.parameters():
+            p.mul_(1.3)
+        answers = top_logits(victim(x.to(DEV)), 3)
+    seen = []
+    atk.grad_probe = lambda it, g: seen.append(g.clone())
+    delta = atk(x, answers)
+    assert delta.shape == x.shape and float(delta.abs().max()) <= 16 / 255 + 1e-7 and float(delta.abs().max()) > 0
+    xx = x.to(DEV).requires_grad_(True)
+    (want,) = torch.autograd.grad(distillation_loss(atk.model(xx), answers), xx)
+    assert (seen[0] - want).norm() <= 1e-4 * want.norm()
+    targeted = ta.load_attack_class("mifgsm")(model_name="toy_cnn", epoch=2, loss="distillation", targeted=True)
+    assert float(targeted(x, [torch.zeros(4, dtype=torch.int64), answers]).abs().max()) <= 16 / 255 + 1e-7

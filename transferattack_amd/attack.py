@@ -369,6 +369,9 @@ class Attack(object):
     def loss_function(self, loss):
         if loss == 'crossentropy':
             return nn.CrossEntropyLoss()
+        if loss == 'distillation':                      # labels are a victim's answers (distill.TopLogits)
+            from .distill import DistillationLoss
+            return DistillationLoss()
         raise Exception("Unsupported loss {}".format(loss))
 
     def transform(self, data, **kwargs):

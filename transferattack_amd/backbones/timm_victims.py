@@ -9,10 +9,12 @@ tests/test_backbones.py: the parameter totals against the published model cards 
 Visformer-S 40.22 M to the digits the cards print) and the key / shape rules of the three layouts.  Normalisation statistics: timm's ``default_cfg`` of all three is the ImageNet
 default, read by ``wrap_model`` (utils.py:44-47)."""
 import math
+import os
 
 import torch
 import torch.nn as nn
 
+from .. import relative
 from .vit import Block as VitBlock, Mlp
 
 IMAGENET_CFG = {"mean": (0.485, 0.456, 0.406), "std": (0.229, 0.224, 0.225)}
@@ -222,8 +224,22 @@ class WindowAttention(nn.Module):
         self.proj = nn.Linear(dim, dim)
         nn.init.trunc_normal_(self.relative_position_bias_table, std=0.02)
 
+    def _buckets(self):
+        """the plan of ``relative_position_index``, built once per device (and again if a checkpoint replaces the index)"""
+        index = self.relative_position_index
+        kept = self.__dict__.get("_ta_buckets")
+        if kept is None or kept[0] is not index or kept[1] != index._version:
+            kept = self.__dict__["_ta_buckets"] = (index, index._version, relative.RelativeBuckets.from_index(index))
+        return kept[2]
+
     def forward(self, x, mask=None):
         bw, n, c = x.shape
+        if x.is_cuda and os.environ.get("TA_RELATIVE_ATTENTION", "0") == "1":
+            # opt-in: scores, bias, mask, softmax and the product with the values as one kernel each way (csrc/nn/
+            # attention_window.hip); the same function with another order of the fp32 sums
+            qkv = self.qkv(x).view(bw, n, 3, self.heads, c // self.heads)
+            return self.proj(relative.relative_attention_packed(qkv, self.relative_position_bias_table, self._buckets(), scale=self.scale,
+                                                                mask=mask))
         q, k, v = self.qkv(x).reshape(bw, n, 3, self.heads, c // self.heads).permute(2, 0, 3, 1, 4)
         attn = (q * self.scale) @ k.transpose(-2, -1)
         bias = self.relative_position_bias_table[self.relative_position_index.view(-1)].view(n, n, -1)

@@ -207,7 +207,10 @@ def _forward(q, k, v, table, out, o, save):
 
 
 def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
-    dtable = torch.zeros_like(table) if table_grad else None
+    dtable = None
+    if table_grad:                                       # rows behind the plan's last bucket are not written
+        covered = table.shape[0] == o.buckets.buckets and out.numel() > 0 and k.shape[2] > 0
+        dtable = torch.empty_like(table) if covered else torch.zeros_like(table)
     if out.numel() == 0 or k.shape[2] == 0:
         for t in (dq, dk, dv):
             t.zero_()
@@ -222,7 +225,7 @@ def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
     a.dv_sb, a.dv_sh, a.dv_sn, _ = dv.stride()
     if dtable is not None:
         a.dtable, a.pair_order, a.pair_starts = dtable.data_ptr(), _nn.ptr(o.buckets.order), _nn.ptr(o.buckets.starts)
-        a.buckets = o.buckets.buckets                    # rows of the table behind the plan's last bucket: their gradient stays 0
+        a.buckets = o.buckets.buckets
     ws = _workspace(a, q, True)
     _nn._launch("ta_nn_attention_backward", q, a)
     del ws
