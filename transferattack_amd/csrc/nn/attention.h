@@ -143,19 +143,26 @@ template <int SUBS> struct Weights<float, SUBS> {
 // acc[q][dt] += (tile^T)[dim 16 dt + ..][row] * w[q][row][column], over the rows
 template <int DP, int NQ, int SUBS, class T>
 __device__ __forceinline__ void mma_transposed(const T* lds, const Weights<T, SUBS> (&w)[NQ], f32x4 (&acc)[NQ][DP / 16], int c, int g) {
+    // operands of one group of products are read while the last group's are multiplied
     if constexpr (sizeof(T) == 4) {
+        float a[2][4][DP / 16];
+        auto read = [&](int t) {
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t)
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float* p = lds + (16 * t + 4 * g + r) * Tile<T, DP>::LD + c;
+                for (int dt = 0; dt < DP / 16; ++dt) a[t & 1][r][dt] = lds[(16 * t + 4 * g + r) * Tile<T, DP>::LD + c + 16 * dt];
+        };
+        read(0);
 #pragma unroll
-                for (int dt = 0; dt < DP / 16; ++dt) {
-                    const float a = p[16 * dt];
+        for (int t = 0; t < SUBS; ++t) {
+            if (t + 1 < SUBS) read(t + 1);
 #pragma unroll
-                    for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(a, w[q].v[t][r], acc[q][dt]);
-                }
-            }
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) acc[q][dt] = mfma(a[t & 1][r][dt], w[q].v[t][r], acc[q][dt]);
+        }
     } else {
 #pragma unroll
         for (int s = 0; s < SUBS / 2; ++s)
@@ -383,14 +390,19 @@ inline int biases_of(const AttentionArgs& a) { return a.mask_kind || !a.bias_in_
 inline bool is_window(const ta_nn_attention_args& a) {
     return a.m <= 64 && a.n <= 64 && a.dim <= 64 && a.heads == a.kv_heads && !a.key_lengths && !a.query_start;
 }
-// workgroups per head of its backward pass, each with sequences of one mask: enough to fill the CUs twice, as they hold them
 inline int window_periods(const ta_nn_attention_args& a) { return a.mask_kind ? a.mask_period : 1; }
-inline int window_parts(const ta_nn_attention_args& a, int64_t workgroups) {
-    const int64_t classes = window_periods(a), most = ceil_div(a.batch, classes);
-    const int64_t wanted = ceil_div(workgroups, classes * a.heads);
-    return static_cast<int>(wanted < most ? wanted : most);
+// Parts that the sequences of one head and mask are divided into, a workgroup each: what takes the fewest rounds of sequences when
+// `slots` workgroups run at once (a part costs half a sequence by itself).
+inline int window_parts(const ta_nn_attention_args& a, bool backward) {
+    const int64_t slots = backward ? 512 : 768;          // two and three to a CU, by the registers they take
+    const int64_t classes = static_cast<int64_t>(window_periods(a)) * a.heads, most = ceil_div(a.batch, window_periods(a));
+    int64_t best = 1, least = INT64_MAX;
+    for (int64_t p = 1; p <= most && (p - 1) * classes < 4 * slots; ++p) {
+        const int64_t cost = ceil_div(classes * p, slots) * (2 * ceil_div(most, p) + 1);
+        if (cost < least) least = cost, best = p;
+    }
+    return static_cast<int>(best);
 }
-constexpr int kWindowWorkgroups = 1024;
 int launch_window(AttentionArgs a, bool backward, hipStream_t st);
 
 // Few queries against many keys -- the next token of every sequence: attention_few.hip.

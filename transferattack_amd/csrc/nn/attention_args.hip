@@ -5,7 +5,7 @@ namespace ta_nn {
 
 // batch chunks of the table's gradient: enough workgroups to fill 256 CUs a few times over, a chunk never without a sequence
 static int table_chunks(const ta_nn_attention_args& a) {
-    if (is_window(a)) return window_parts(a, kWindowWorkgroups) * window_periods(a);
+    if (is_window(a)) return window_parts(a, true) * window_periods(a);
     const int64_t tiles = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads;
     const int64_t wanted = ceil_div(2048, tiles);
     return static_cast<int>(wanted < a.batch ? wanted : a.batch);

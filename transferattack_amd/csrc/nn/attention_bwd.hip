@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = exp2_hw(s[t][r] - top) * inv, dp = p == 0.0f ? 0.0f : ds[0][t][r];      // a masked value may be anything
+                const float p = exp2_hw(s[t][r] - top) * inv, dp = ds[0][t][r];
                 ds[0][t][r] = p * (dp - delta);
                 exact += p * dp;
             }
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
             for (int r = 0; r < 4; ++r) {
                 const float w = exp2_hw(p[0][t][r] - top[r]) * inv[r];
                 p[0][t][r] = w;
-                ds[0][t][r] = w == 0.0f ? 0.0f : w * (ds[0][t][r] - delta[r]);
+                ds[0][t][r] = w * (ds[0][t][r] - delta[r]);
             }
         }
         mma_transposed<DP, 1, SUBS>(gs, p, dv, c, g);
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float p = valid ? exp2_hw(s[t][r] - top) * inv : 0.0f;
-                sum[t][r] += p == 0.0f ? 0.0f : p * (dp[t][r] - delta);
+                sum[t][r] += p * (dp[t][r] - delta);
             }
         });
     }

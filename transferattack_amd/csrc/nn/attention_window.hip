@@ -53,8 +53,6 @@ __device__ __forceinline__ void window_bias(const AttentionArgs& a, const Share&
     }
 }
 
-__device__ __forceinline__ float added(float s, float c, float add) { return add == -INFINITY ? -INFINITY : fmaf(s, c, add); }
-
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void window_fwd(AttentionArgs a, int parts) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, TILE = 64 * Tile<T, DP>::LD;
@@ -102,7 +100,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd(AttentionArgs a, int parts)
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[0][t][r] = added(s[0][t][r], scale, add[t][r]);
+                s[0][t][r] = fmaf(s[0][t][r], scale, add[t][r]);
                 top = fmaxf(top, s[0][t][r]);
             }
         top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); });
@@ -198,8 +196,8 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[t][r] = exp2_hw(added(p[t][r], scale, add[t][r]) - top) * inv;
-                    delta += p[t][r] == 0.0f ? 0.0f : p[t][r] * ds[0][t][r];      // sum_j p dp is out . grad, unrounded
+                    p[t][r] = exp2_hw(fmaf(p[t][r], scale, add[t][r]) - top) * inv;
+                    delta += p[t][r] * ds[0][t][r];                               // sum_j p dp is out . grad, unrounded
                 }
             delta = reduce_rows(delta, Sum{});
 #pragma unroll
@@ -207,7 +205,7 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float w = p[t][r];
-                    ds[0][t][r] = w == 0.0f ? 0.0f : w * (ds[0][t][r] - delta);
+                    ds[0][t][r] = w * (ds[0][t][r] - delta);
                     table_sum[t][r] += ds[0][t][r];
                     ps[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(w);
                     dss[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(ds[0][t][r]);
@@ -255,7 +253,7 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
 }
 
 template <class T, int DP> int launch_window_by(AttentionArgs a, bool backward, hipStream_t st) {
-    const int parts = window_parts(a, kWindowWorkgroups);
+    const int parts = window_parts(a, backward);
     const int64_t blocks = static_cast<int64_t>(a.heads) * window_periods(a) * parts;
     TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many windows for one launch");
     const size_t tile = 64 * Tile<T, DP>::LD * sizeof(T);
