@@ -47,9 +47,10 @@ const char* ta_nn_last_error(void);
  * A query that sees no key gives zeros, and zero gradients. */
 typedef struct ta_nn_attention_args {
     int dtype;                                   /* of q, k, v, out, grad, dq, dk, dv */
-    int batch, heads, kv_heads, m, n, dim;       /* m queries, n keys; heads a multiple of kv_heads; dim <= 128 */
+    int batch, heads, kv_heads, m, n, dim;       /* m queries, n keys; heads a multiple of kv_heads; dim <= 128,
+                                                    16 bytes or a multiple of that */
     const void *q, *k, *v;
-    int64_t q_sb, q_sh, q_sm, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;
+    int64_t q_sb, q_sh, q_sm, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn;      /* token strides (_sm, _sn): 0 .. 2^23 - 1 */
     float scale;
     int table_dtype, buckets;
     const void* table;                           /* [buckets][heads], contiguous */

@@ -17,6 +17,8 @@ struct AttentionArgs : ta_nn_attention_args {
     int bias_in_lds;                                     // the bias values of a block's heads are staged in LDS
     float* delta;                                        // [batch][heads][m]: sum_d out grad
     float* partial;                                      // sums of score gradients, per batch chunk
+    float* far;                                          // distances: [batch][heads][64 queries][2] sums past either end
+    float* by_distance;                                  // distances: [heads][64 (tile difference)][128] sums of the near tiles
     int chunks;
 };
 
@@ -48,33 +50,32 @@ __device__ __forceinline__ f32x4 mma_row(half8 a, half8 b, f32x4 c) { return mfm
 // rows of a tile over 16: as many as leave the accumulators their registers
 template <int DP> constexpr int kSubs = DP <= 64 ? 4 : 2;
 
-// LDS tile: ROWS rows of DP elements, rows 16 bytes longer than they need to be so that the 16 rows of a fragment start in
-// different banks
+// Elements between rows of an LDS tile: 16-bit rows start 8 of the 64 banks further on than a multiple of them, so that what reads
+// a tile transposed -- 16 lanes four rows of 32 bytes -- meets no bank twice; what reads it by rows (16 lanes a row each, 16 bytes)
+// meets each twice.  With 4 banks instead, the other way round: 8191 keys in fp16 507 us (455 with 8), 1023 padded tokens in bf16
+// forward 64, backward 81 + 105 us (59, 71 + 91 with 8).
 template <class T, int DP> struct Tile {
-    static constexpr int LD = DP + 16 / static_cast<int>(sizeof(T));
-    static constexpr int LOADS(int rows, int threads) { return (rows * DP / Frag<T>::VE + threads - 1) / threads; }
+    static constexpr int LD = DP + (sizeof(T) == 2 ? 16 : 4);
 };
 
-// ROWS x DP elements from memory into registers (zero past `rows` and `dim`); `put` moves them to LDS one barrier later.
-// `base`: row 0, the same for the workgroup; a row is less than 2^24 elements behind the last
+// ROWS x DP elements from memory into registers (zero past `rows` and `dim`, a multiple of a vector); `put` moves them to LDS one
+// barrier later.  `base`: row 0, the same for the workgroup; a row is less than 2^23 elements behind the last
 template <class T, int DP, int ROWS, int THREADS> struct Staged {
     static constexpr int VE = Frag<T>::VE, PER_ROW = DP / VE, COUNT = (ROWS * PER_ROW + THREADS - 1) / THREADS;
     __device__ __forceinline__ static bool mine(int e) { return (ROWS * PER_ROW) % THREADS == 0 || e < ROWS * PER_ROW; }
     Vec<T> v[COUNT];
     __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int dim) {
-        const int step = static_cast<int>(stride);
-        if (rows >= ROWS && dim == DP) {
+        const unsigned step = static_cast<unsigned>(stride);
+        const bool whole = rows >= ROWS && dim == DP;
 #pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
-                if (mine(e)) v[i] = load_vec(base + (r * step + d));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < COUNT; ++i) {
-                const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
+        for (int i = 0; i < COUNT; ++i) {
+            const int e = static_cast<int>(threadIdx.x) + i * THREADS, r = e / PER_ROW, d = e % PER_ROW * VE;
+            const unsigned offset = (r * step + d) * static_cast<unsigned>(sizeof(T));
+            if (whole) {
+                if (mine(e)) v[i] = load_at(base, offset);
+            } else {
                 v[i].raw = u32x4{0, 0, 0, 0};
-                if (mine(e) && r < rows && d < dim) v[i] = load_part(base + (r * step + d), dim - d);
+                if (mine(e) && r < rows && d < dim) v[i] = load_at(base, offset);
             }
         }
     }
@@ -97,7 +98,7 @@ template <class T> __device__ __forceinline__ typename Frag<T>::Row row_frag_glo
     const int d = dc * Frag<T>::D + g * Frag<T>::VE;
     Vec<T> v;
     v.raw = u32x4{0, 0, 0, 0};
-    if (valid && d < dim) v = load_part(p + d, dim - d);
+    if (valid && d < dim) v = load_vec(p + d);
     return __builtin_bit_cast(typename Frag<T>::Row, v);
 }
 
@@ -260,6 +261,20 @@ enum Kind {
     kEdge                                                // whatever there is
 };
 
+// Whether all distances of a tile of 64 keys lie past the same end (and which: -1 the first, 1 the last entry): the table's
+// gradient then needs but the sum of the tile.  `low`, `high`: the lowest and the highest entry.
+__host__ __device__ inline int far_end(const AttentionArgs& a, int64_t low, int64_t high) { return high <= 0 ? -1 : low >= a.distances - 1 ? 1 : 0; }
+// the key tiles that are not so for queries i0 .. i0 + 63 (all sequences begin at the same position): the first, and how many at most
+__host__ __device__ inline int near_tiles(const AttentionArgs& a) {
+    const int tiles = (a.n + 63) / 64, most = (a.distances + 125) / 64 + 1;
+    return tiles < most ? tiles : most;
+}
+__device__ __forceinline__ int first_near_tile(const AttentionArgs& a, int i0) {
+    const int64_t after = static_cast<int64_t>(a.start) + i0 + a.first - 63;       // tile t is past the first entry if 64 t > after
+    const int64_t t = after < 0 ? 0 : after / 64 + 1, last = (a.n + 63) / 64 - near_tiles(a);
+    return static_cast<int>(t < last ? t : last);
+}
+
 // `low`, `high`: the lowest and the highest entry of the distances in the tile
 template <int BIASES> __device__ __forceinline__ Kind tile_kind(const AttentionArgs& a, bool all_seen, bool one_head, int64_t low, int64_t high) {
     if (BIASES == kAny || !all_seen) return kEdge;
@@ -344,13 +359,7 @@ template <class T, int DP> __device__ __forceinline__ void store_column(T* p, co
         T v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = from_float<T>(o[t][r] * f);
-        if (d + 4 <= dim) {
-            __builtin_memcpy(p + d, v, sizeof(v));
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (d + r < dim) p[d + r] = v[r];
-        }
+        if (d < dim) __builtin_memcpy(p + d, v, sizeof(v));
     }
 }
 
@@ -387,21 +396,24 @@ inline size_t bias_lds_bytes(AttentionArgs& a, int64_t columns, int pad = kPad) 
 inline int biases_of(const AttentionArgs& a) { return a.mask_kind || !a.bias_in_lds ? kAny : a.distances ? kByDistance : kByPair; }
 
 // Many short sequences whose pairs are the same in all of them (or in every mask_period-th): attention_window.hip.
-inline bool is_window(const ta_nn_attention_args& a) {
+__host__ __device__ inline bool is_window(const ta_nn_attention_args& a) {
     return a.m <= 64 && a.n <= 64 && a.dim <= 64 && a.heads == a.kv_heads && !a.key_lengths && !a.query_start;
 }
 inline int window_periods(const ta_nn_attention_args& a) { return a.mask_kind ? a.mask_period : 1; }
-// Parts that the sequences of one head and mask are divided into, a workgroup each: what takes the fewest rounds of sequences when
-// `slots` workgroups run at once (a part costs half a sequence by itself).
-inline int window_parts(const ta_nn_attention_args& a, bool backward) {
-    const int64_t slots = backward ? 512 : 768;          // two and three to a CU, by the registers they take
-    const int64_t classes = static_cast<int64_t>(window_periods(a)) * a.heads, most = ceil_div(a.batch, window_periods(a));
+// Parts to divide `count` sequences into, each a workgroup of `classes` kinds: what takes the fewest rounds of sequences when `slots`
+// workgroups run at once (a part costs half a sequence by itself).
+inline int balanced_parts(int64_t classes, int64_t count, int64_t slots) {
     int64_t best = 1, least = INT64_MAX;
-    for (int64_t p = 1; p <= most && (p - 1) * classes < 4 * slots; ++p) {
-        const int64_t cost = ceil_div(classes * p, slots) * (2 * ceil_div(most, p) + 1);
+    for (int64_t p = 1; p <= count && (p - 1) * classes < 4 * slots; ++p) {
+        const int64_t cost = ceil_div(classes * p, slots) * (2 * ceil_div(count, p) + 1);
         if (cost < least) least = cost, best = p;
     }
     return static_cast<int>(best);
+}
+// Parts that the sequences of one head and mask are divided into, a workgroup each.
+inline int window_parts(const ta_nn_attention_args& a, bool backward) {
+    return balanced_parts(static_cast<int64_t>(window_periods(a)) * a.heads, ceil_div(a.batch, window_periods(a)),
+                          backward ? 512 : 768);         // two and three to a CU, by the registers they take
 }
 int launch_window(AttentionArgs a, bool backward, hipStream_t st);
 

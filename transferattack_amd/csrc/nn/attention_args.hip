@@ -3,25 +3,40 @@
 
 namespace ta_nn {
 
-// batch chunks of the table's gradient: enough workgroups to fill 256 CUs a few times over, a chunk never without a sequence
-static int table_chunks(const ta_nn_attention_args& a) {
+// tiles of 64 queries x 64 keys whose score gradients the table's gradient needs one by one
+static int64_t table_tiles(const AttentionArgs& a) { return ceil_div(a.m, 64) * (a.distances ? near_tiles(a) : ceil_div(a.n, 64)); }
+
+static int table_chunks(const AttentionArgs& a) {
     if (is_window(a)) return window_parts(a, true) * window_periods(a);
-    const int64_t tiles = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads;
-    const int64_t wanted = ceil_div(2048, tiles);
-    return static_cast<int>(wanted < a.batch ? wanted : a.batch);
+    return balanced_parts(table_tiles(a) * a.heads, a.batch, 512);
 }
 
-int64_t workspace_floats(const ta_nn_attention_args& a, bool backward) {
-    if (!backward) {
-        const int splits = is_few(a) ? few_splits(a) : 1;
-        return splits == 1 ? 0 : static_cast<int64_t>(a.batch) * a.kv_heads * splits * (32 + 16 * a.dim);
-    }
+// backward: delta, then the table's partial sums, then (distances) the sums past the ends and the sums by distance
+static int64_t layout(AttentionArgs& a) {
     int64_t floats = static_cast<int64_t>(a.batch) * a.heads * a.m;
-    if (a.dtable) {
-        const int64_t per_chunk = a.distances ? ceil_div(a.m, 64) * ceil_div(a.n, 64) * 128 : static_cast<int64_t>(a.m) * a.n;
-        floats += per_chunk * a.heads * table_chunks(a);
+    a.delta = a.workspace;
+    if (a.dtable == nullptr) return floats;
+    a.chunks = table_chunks(a);
+    const int64_t per_chunk = a.distances ? table_tiles(a) * 128 : static_cast<int64_t>(a.m) * a.n;
+    a.partial = a.workspace + floats;
+    floats += per_chunk * a.heads * a.chunks;
+    if (a.distances) {
+        a.far = a.workspace + floats;
+        floats += static_cast<int64_t>(a.batch) * a.heads * ceil_div(a.m, 64) * 2;
+        a.by_distance = a.workspace + floats;
+        floats += a.heads * (ceil_div(a.m, 64) + ceil_div(a.n, 64) - 1) * 128;
     }
     return floats;
+}
+
+int64_t workspace_floats(const ta_nn_attention_args& args, bool backward) {
+    if (!backward) {
+        const int splits = is_few(args) ? few_splits(args) : 1;
+        return splits == 1 ? 0 : static_cast<int64_t>(args.batch) * args.kv_heads * splits * (32 + 16 * args.dim);
+    }
+    AttentionArgs a{};
+    static_cast<ta_nn_attention_args&>(a) = args;
+    return layout(a);
 }
 
 int check_attention(const ta_nn_attention_args* args, AttentionArgs& a) {
@@ -34,6 +49,7 @@ int check_attention(const ta_nn_attention_args* args, AttentionArgs& a) {
     TA_NN_REQUIRE(a.m < (1 << 30) && a.n < (1 << 30) && a.distances < (1 << 29), "more than 2^30 tokens");
     TA_NN_REQUIRE(a.heads % a.kv_heads == 0, "%d heads do not share %d key heads evenly", a.heads, a.kv_heads);
     TA_NN_REQUIRE(a.dim >= 1 && a.dim <= 128, "head dimension %d (1 .. 128)", a.dim);
+    TA_NN_REQUIRE(a.dim % (a.dtype == TA_NN_F32 ? 4 : 8) == 0, "head dimension %d is not a multiple of 16 bytes", a.dim);
     TA_NN_REQUIRE(a.q && a.k && a.v && a.table && a.index && a.out, "null pointer");
     TA_NN_REQUIRE(a.buckets >= 1 && a.buckets <= 65536, "%d buckets", a.buckets);
     TA_NN_REQUIRE(a.distances >= 0, "%d distances", a.distances);
@@ -45,8 +61,8 @@ int check_attention(const ta_nn_attention_args* args, AttentionArgs& a) {
     TA_NN_REQUIRE(a.mask_kind == TA_NN_MASK_NONE || (a.mask && a.mask_period >= 1), "mask period %d", a.mask_period);
     const int64_t steps[] = {a.q_sm, a.k_sn, a.v_sn, a.g_sm};
     for (int64_t step : steps)
-        TA_NN_REQUIRE(step > -(1 << 24) && step < (1 << 24), "token stride %lld (below 2^24 elements)", static_cast<long long>(step));
-    a.chunks = table_chunks(a);
+        TA_NN_REQUIRE(step >= 0 && step < (1 << 23), "token stride %lld (below 2^23 elements)", static_cast<long long>(step));
+    layout(a);
     return 0;
 }
 

@@ -10,8 +10,8 @@
 namespace ta_nn {
 
 template <class T, int DP, int BIASES>
-__global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_q(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = sizeof(T) == 2 ? 2 : kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
     T* vs = ks + ROWS * Tile<T, DP>::LD;
@@ -57,6 +57,9 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
     // delta for this kernel is out . grad.  For 16-bit tensors out is rounded, and so were the probabilities it was made with; for
     // the table, whose gradient is a sum of differences that nearly cancel, and for the keys it is taken anew: sum_j p_ij dp_ij.
     float exact = 0.0f;
+    // sums past either end of the distances, for the table: of p and of p dp, since delta is not known yet
+    float far_p[2] = {0.0f, 0.0f}, far_dp[2] = {0.0f, 0.0f};
+    const bool wants_far = BIASES != kByPair && a.far != nullptr;
     f32x4 dq[1][DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -88,25 +91,54 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_q(AttentionArgs a) {
             }
         }
         score_tile<BIASES, decltype(tag)::kind, false>(a, col, j0, g, s);
+        float exact_tile = 0.0f;
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float p = exp2_hw(s[t][r] - top) * inv, dp = ds[0][t][r];
                 ds[0][t][r] = p * (dp - delta);
-                exact += p * dp;
+                s[t][r] = p;
+                exact_tile += p * dp;
             }
+        exact += exact_tile;
+        if constexpr (BIASES != kByPair && decltype(tag)::kind != kNear) {
+            const int64_t j64 = j0 & ~63;
+            const int end = wants_far ? far_end(a, j64 - pos1 - a.first, j64 + 63 - pos0 - a.first) : 0;
+            if (end != 0) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum += s[t][r];
+                far_p[0] += end < 0 ? sum : 0.0f;
+                far_p[1] += end > 0 ? sum : 0.0f;
+                far_dp[0] += end < 0 ? exact_tile : 0.0f;
+                far_dp[1] += end > 0 ? exact_tile : 0.0f;
+            }
+        }
         mma_transposed<DP, 1, SUBS>(ks, ds, dq, c, g);
         });
     }
     exact = reduce_rows(exact, Sum{});
     if (valid && g == 0) a.delta[at] = exact;
+    if (BIASES != kByPair && wants_far) {
+        __shared__ float far_lds[4][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float sum = wave_sum(valid ? far_dp[e] - exact * far_p[e] : 0.0f);
+            if ((tid & 63) == 0) far_lds[wave][e] = sum;
+        }
+        __syncthreads();
+        if (tid < 2)
+            a.far[((b * a.heads + head) * tiles + i0 / 64) * 2 + tid] = far_lds[0][tid] + far_lds[1][tid] + far_lds[2][tid] + far_lds[3][tid];
+    }
     if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
 }
 
 template <class T, int DP, int BIASES>
-__global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
-    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS;
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_kv(AttentionArgs a) {
+    constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = sizeof(T) == 2 ? 2 : kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* qs = reinterpret_cast<T*>(smem);
     T* gs = qs + ROWS * Tile<T, DP>::LD;
@@ -217,7 +249,7 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_kv(AttentionArgs a) {
 }
 
 // ds of one tile of 64 queries x 64 keys of a head, summed over the sequences of a chunk.  Pairs: the tile as it is; distances:
-// its 127 diagonals (the distance is the same along each).
+// its 127 diagonals (the distance is the same along each), and only tiles that are not past an end altogether.
 template <class T, int DP, int BIASES>
 __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D;
@@ -227,12 +259,12 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     float* bias_lds = reinterpret_cast<float*>(vs + 64 * Tile<T, DP>::LD);
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
-    const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64;
+    const int q_tiles = (a.m + 63) / 64, k_tiles = a.distances ? near_tiles(a) : (a.n + 63) / 64;
     const int64_t block = blockIdx.x;
     const int k_tile = static_cast<int>(block % k_tiles), q_tile = static_cast<int>(block / k_tiles % q_tiles);
     const int head = static_cast<int>(block / k_tiles / q_tiles % a.heads);
     const int chunk = static_cast<int>(block / k_tiles / q_tiles / a.heads);
-    const int i0 = q_tile * 64, j0 = k_tile * 64, hk = head / group;
+    const int i0 = q_tile * 64, j0 = (a.distances ? first_near_tile(a, i0) + k_tile : k_tile) * 64, hk = head / group;
     const bool valid = i0 + 16 * wave + c < a.m;
     const int query = min(i0 + 16 * wave + c, a.m - 1);
     if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
@@ -249,6 +281,8 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
             keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
         }
         if (j0 >= keys) continue;                        // (the same for the whole workgroup)
+        if (a.distances && far_end(a, j0 - (static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1) - a.first,
+                                   j0 + 63 - (static_cast<int64_t>(start) + i0) - a.first) != 0) continue;      // in attention_bwd_q's sums
         const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
         const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
         Staged<T, DP, 64, 256> kr, vr;
@@ -333,7 +367,23 @@ __global__ __launch_bounds__(256) void attention_pair_sums(AttentionArgs a) {
         a.partial[head * pairs + pair] = static_cast<float>(red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane]);
 }
 
-// one workgroup for each bucket and head: the partial sums in a fixed order, in 64 bits
+// Distances, first: the near tiles' diagonals by distance.  A workgroup has one head and one difference between the numbers of key
+// and query tile; thread t adds diagonal t of all such tiles and chunks, in order, in 64 bits.
+__global__ __launch_bounds__(128) void attention_distance_sums(AttentionArgs a) {
+    const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64, near = near_tiles(a), offsets = q_tiles + k_tiles - 1;
+    const int head = static_cast<int>(blockIdx.x) / offsets, offset = static_cast<int>(blockIdx.x) % offsets - (q_tiles - 1);
+    double sum = 0.0;
+    for (int q = max(0, -offset); q < q_tiles && q + offset < k_tiles; ++q) {
+        const int at = is_window(a) ? 0 : q + offset - first_near_tile(a, 64 * q);
+        if (at < 0 || at >= near) continue;
+#pragma unroll 4
+        for (int chunk = 0; chunk < a.chunks; ++chunk)
+            sum += a.partial[(((static_cast<int64_t>(chunk) * a.heads + head) * q_tiles + q) * near + at) * 128 + threadIdx.x];
+    }
+    a.by_distance[static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x] = static_cast<float>(sum);
+}
+
+// one workgroup for each bucket and head: the sums of its pairs or distances in a fixed order, in 64 bits
 __global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
     __shared__ double red[4];
     const int bucket = static_cast<int>(blockIdx.x) / a.heads, head = static_cast<int>(blockIdx.x) % a.heads;
@@ -343,14 +393,19 @@ __global__ __launch_bounds__(256) void attention_table_sums(AttentionArgs a) {
         const int from = a.pair_starts[bucket], to = a.pair_starts[bucket + 1];
         for (int e = from + static_cast<int>(threadIdx.x); e < to; e += 256) sum += a.partial[head * pairs + a.pair_order[e]];
     } else {
-        const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64;
-        const int64_t entries = static_cast<int64_t>(q_tiles) * k_tiles * 128;
-        for (int64_t e = threadIdx.x; e < entries; e += 256) {
-            const int t = static_cast<int>(e & 127), k_tile = static_cast<int>(e / 128 % k_tiles), q_tile = static_cast<int>(e / 128 / k_tiles);
-            const int64_t d = static_cast<int64_t>(k_tile - q_tile) * 64 + t - 63 - a.start - a.first;
+        const int q_tiles = (a.m + 63) / 64, k_tiles = (a.n + 63) / 64, offsets = q_tiles + k_tiles - 1;
+        const int* index = static_cast<const int*>(a.index);
+        for (int e = threadIdx.x; e < offsets * 128; e += 256) {
+            const int64_t d = static_cast<int64_t>(e / 128 - (q_tiles - 1)) * 64 + (e & 127) - 63 - a.start - a.first;
             const int at = d < 0 ? 0 : d >= a.distances ? a.distances - 1 : static_cast<int>(d);
-            if (static_cast<const int*>(a.index)[at] != bucket) continue;
-            for (int chunk = 0; chunk < a.chunks; ++chunk) sum += a.partial[(static_cast<int64_t>(chunk) * a.heads + head) * entries + e];
+            if (index[at] == bucket) sum += a.by_distance[static_cast<int64_t>(head) * offsets * 128 + e];
+        }
+        if (!is_window(a)) {
+            const int64_t rows = static_cast<int64_t>(a.batch) * q_tiles;
+            for (int end = 0; end < 2; ++end)
+                if (index[end == 0 ? 0 : a.distances - 1] == bucket)
+                    for (int64_t e = threadIdx.x; e < rows; e += 256)
+                        sum += a.far[((e / q_tiles * a.heads + head) * q_tiles + e % q_tiles) * 2 + end];
         }
     }
     sum = block_sum<4>(sum, red);
@@ -362,6 +417,10 @@ int launch_table_sums(const AttentionArgs& a, hipStream_t st) {
         const int64_t blocks = ceil_div(static_cast<int64_t>(a.m) * a.n, 64) * a.heads;
         TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "%d x %d pairs", a.m, a.n);
         hipLaunchKernelGGL(attention_pair_sums, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a);
+    } else {
+        const int64_t blocks = (ceil_div(a.m, 64) + ceil_div(a.n, 64) - 1) * a.heads;
+        TA_NN_REQUIRE(blocks * 128 <= 0x7FFFFFFF, "%d x %d tokens", a.m, a.n);
+        hipLaunchKernelGGL(attention_distance_sums, dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, a);
     }
     hipLaunchKernelGGL(attention_table_sums, dim3(static_cast<unsigned>(a.buckets) * a.heads), dim3(256), 0, st, a);
     return check_launch("ta_nn_attention_backward");
@@ -371,7 +430,7 @@ template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) 
     const size_t tiles = 2 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T), table_tiles = 2 * 64 * Tile<T, DP>::LD * sizeof(T);
     const size_t bias = bias_lds_bytes(a, 1);
     const int64_t q_blocks = ceil_div(a.m, 64) * a.heads * a.batch, k_blocks = ceil_div(a.n, 64) * a.kv_heads * a.batch;
-    const int64_t t_blocks = ceil_div(a.m, 64) * ceil_div(a.n, 64) * a.heads * a.chunks;
+    const int64_t t_blocks = ceil_div(a.m, 64) * (a.distances ? near_tiles(a) : ceil_div(a.n, 64)) * a.heads * a.chunks;
     TA_NN_REQUIRE(q_blocks <= 0x7FFFFFFF && k_blocks <= 0x7FFFFFFF && t_blocks <= 0x7FFFFFFF, "too many tokens for one launch");
     TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_q<T, DP, BIASES>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a));
     TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_kv<T, DP, BIASES>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), tiles + 3 * 64 * 4 + bias, st, a));
@@ -398,8 +457,6 @@ extern "C" int ta_nn_attention_backward(const ta_nn_attention_args* args, void* 
     }
     TA_NN_REQUIRE(!(a.dtable && a.query_start && a.distances), "the table's gradient needs one position of query 0 for all sequences");
     TA_NN_REQUIRE(static_cast<int64_t>(a.buckets) * a.heads <= 0x7FFFFFFF, "%d buckets, %d heads", a.buckets, a.heads);
-    a.delta = a.workspace;
-    a.partial = a.workspace + static_cast<int64_t>(a.batch) * a.heads * a.m;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (ta_nn::is_window(a)) {
         if (int rc = ta_nn::launch_window(a, true, st)) return rc;

@@ -36,7 +36,8 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
     const int own = valid ? c : columns - 1, head = hk * group + own / a.m, query = own % a.m;
     const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
     const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-    const int k_step = static_cast<int>(a.k_sn), v_step = static_cast<int>(a.v_sn);
+    const unsigned k_step = static_cast<unsigned>(a.k_sn), v_step = static_cast<unsigned>(a.v_sn);
+    constexpr unsigned ES = sizeof(T);
     typename Frag<T>::Row k[SUBS][DC];
     Vec<T> v[LOADS];
     auto fetch = [&](int j0) {
@@ -48,11 +49,11 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
             for (int t = 0; t < SUBS; ++t)
 #pragma unroll
                 for (int dc = 0; dc < DC; ++dc)
-                    k[t][dc] = __builtin_bit_cast(typename Frag<T>::Row, load_vec(kp + ((16 * t + c) * k_step + dc * Frag<T>::D + g * VE)));
+                    k[t][dc] = __builtin_bit_cast(typename Frag<T>::Row, load_at(kp, ((16 * t + c) * k_step + dc * Frag<T>::D + g * VE) * ES));
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int e = lane + 64 * i;
-                v[i] = load_vec(vp + (e / PER_ROW * v_step + e % PER_ROW * VE));
+                v[i] = load_at(vp, (e / PER_ROW * v_step + e % PER_ROW * VE) * ES);
             }
         } else {
 #pragma unroll
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
             for (int i = 0; i < LOADS; ++i) {
                 const int e = lane + 64 * i, r = e / PER_ROW, d = e % PER_ROW * VE;
                 v[i].raw = u32x4{0, 0, 0, 0};
-                if (j0 + r < end && d < a.dim) v[i] = load_part(vp + (r * v_step + d), a.dim - d);
+                if (j0 + r < end && d < a.dim) v[i] = load_at(vp, (r * v_step + d) * ES);
             }
         }
     };

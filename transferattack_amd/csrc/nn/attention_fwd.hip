@@ -9,27 +9,32 @@ constexpr float kSlack = 8.0f;
 // tiles) against every key they see, a tile at a time.  Two tiles in LDS: while one is worked on, the next arrives in registers
 // and is put into the other's place, with one barrier a tile.
 template <class T, int DP, int NQ, int BIASES>
-__global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 3 : 2) void attention_fwd(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = kSubs<DP>, ROWS = 16 * SUBS, TILE = ROWS * Tile<T, DP>::LD;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* tiles = reinterpret_cast<T*>(smem);               // [2][keys, values][ROWS][LD]
     float* bias_lds = reinterpret_cast<float*>(tiles + 4 * TILE);
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
+    // Columns: the group's queries head by head; a tile of them never spans heads where one has as many (tiles that span heads, whose
+    // queries stand far apart, take the slow kind of tile throughout)
     const int64_t columns = static_cast<int64_t>(group) * a.m;
-    const int col_tiles = static_cast<int>((columns + 64 * NQ - 1) / (64 * NQ));
+    const bool by_head = a.m >= 64 * NQ;
+    const int per_head = (a.m + 64 * NQ - 1) / (64 * NQ);
     // workgroups go to the XCDs in turn: with sequence and head as the fastest index an XCD's L2 holds few heads' keys and values
     const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.kv_heads) * a.batch;
     const int hk = static_cast<int>(block % lanes % a.kv_heads);
     const int64_t b = block % lanes / a.kv_heads;
-    int tile = static_cast<int>(block / lanes);
-    if (a.causal) {                                      // the longest begin: the last queries of every head
-        const int per_head = col_tiles / group;
-        tile = per_head * group == col_tiles ? tile % group * per_head + per_head - 1 - tile / group : col_tiles - 1 - tile;
+    const int tile = static_cast<int>(block / lanes);
+    int64_t col0, col1;
+    if (by_head) {                                       // causal: the longest begin, the last queries of every head
+        const int h = tile % group, i0 = (a.causal ? per_head - 1 - tile / group : tile / group) * 64 * NQ;
+        col0 = static_cast<int64_t>(h) * a.m + i0;
+        col1 = static_cast<int64_t>(h) * a.m + min(i0 + 64 * NQ, a.m) - 1;
+    } else {
+        col0 = static_cast<int64_t>(tile) * 64 * NQ;
+        col1 = min(col0 + 64 * NQ, columns) - 1;
     }
-
-    const int64_t col0 = static_cast<int64_t>(tile) * 64 * NQ;
-    const int64_t col1 = min(col0 + 64 * NQ, columns) - 1;
     const int h0 = static_cast<int>(col0 / a.m), h1 = static_cast<int>(col1 / a.m);
     const int start = a.query_start ? a.query_start[b] : a.start;
     // positions of the block's first and last query (of any, where it spans heads)
@@ -58,8 +63,8 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
         const int64_t at = col0 + (wave * NQ + x) * 16 + c;
-        valid[x] = at < columns;
-        const int64_t own = valid[x] ? at : columns - 1;
+        valid[x] = at <= col1;
+        const int64_t own = valid[x] ? at : col1;
         const int h = static_cast<int>(own / a.m);
         query[x] = static_cast<int>(own - static_cast<int64_t>(h) * a.m);
         const int head = hk * group + h;
@@ -78,12 +83,17 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
         fetch(ROWS);
     }
     __syncthreads();
-    for (int j0 = 0, turn = 0; j0 < keys; j0 += ROWS, turn ^= 1) {
-        const T* ks = tiles + turn * 2 * TILE;
-        const T* vs = ks + TILE;
-        by_kind<BIASES>(tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), h0 == h1, j0 - pos1 - a.first,
-                                          j0 + ROWS - 1 - pos0 - a.first),
-                        [&](auto tag) {
+    auto kind_at = [&](int j0) {
+        return tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), h0 == h1, j0 - pos1 - a.first,
+                                 j0 + ROWS - 1 - pos0 - a.first);
+    };
+    int j0 = 0, turn = 0;
+    while (j0 < keys) {
+        // a loop of its own for a run of tiles of one kind: the accumulators stay where they are from tile to tile
+        by_kind<BIASES>(kind_at(j0), [&](auto tag) {
+          do {
+            const T* ks = tiles + turn * 2 * TILE;
+            const T* vs = ks + TILE;
             f32x4 s[NQ][SUBS];
 #pragma unroll
             for (int t = 0; t < SUBS; ++t) {
@@ -136,14 +146,17 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
                 l[x] += sum;
             }
             mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
+            if (j0 + ROWS < keys) {
+                T* next = tiles + (turn ^ 1) * 2 * TILE; // (everyone has left it: the barrier of the last turn)
+                kr.put(next);
+                vr.put(next + TILE);
+                fetch(j0 + 2 * ROWS);
+            }
+            __syncthreads();
+            j0 += ROWS;
+            turn ^= 1;
+          } while (j0 < keys && kind_at(j0) == decltype(tag)::kind);
         });
-        if (j0 + ROWS < keys) {
-            T* next = tiles + (turn ^ 1) * 2 * TILE;     // (everyone has left it: the barrier of the last turn)
-            kr.put(next);
-            vr.put(next + TILE);
-            fetch(j0 + 2 * ROWS);
-        }
-        __syncthreads();
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
@@ -163,7 +176,8 @@ __global__ __launch_bounds__(256, 2) void attention_fwd(AttentionArgs a) {
 
 template <class T, int DP, int NQ> int launch_forward_by(AttentionArgs a, hipStream_t st) {
     const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
-    const int64_t blocks = ceil_div(columns, 64 * NQ) * a.kv_heads * a.batch;
+    const int64_t tiles = a.m >= 64 * NQ ? ceil_div(a.m, 64 * NQ) * (a.heads / a.kv_heads) : ceil_div(columns, 64 * NQ);
+    const int64_t blocks = tiles * a.kv_heads * a.batch;
     TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
     const size_t lds = 4 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T) + bias_lds_bytes(a, 64 * NQ);
     TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_fwd<T, DP, NQ, BIASES>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a));

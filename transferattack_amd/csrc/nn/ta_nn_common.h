@@ -84,12 +84,10 @@ template <class T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
     __builtin_memcpy(&r.raw, p, 16);
     return r;
 }
-// the first `count` elements at p (as many as there are), the rest 0
-template <class T> __device__ __forceinline__ Vec<T> load_part(const T* p, int count) {
-    if (count >= Vec<T>::N) return load_vec(p);
-    Vec<T> r{u32x4{0, 0, 0, 0}};
-#pragma unroll 1
-    for (int i = 0; i < count; ++i) set_bits_at(r, i, bits_of(p[i]));
+// the same at a byte offset from an address the whole workgroup shares: one 32-bit register to a lane
+template <class T> __device__ __forceinline__ Vec<T> load_at(const T* base, unsigned offset) {
+    Vec<T> r;
+    __builtin_memcpy(&r.raw, reinterpret_cast<const char*>(base) + offset, 16);
     return r;
 }
 template <class T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) { __builtin_memcpy(p, &r.raw, 16); }

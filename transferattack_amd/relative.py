@@ -285,16 +285,21 @@ class _PackedAttention(torch.autograd.Function):
 
 
 def _dense_rows(t, token=2):
-    """as the kernels take it: the innermost dimension dense, tokens less than 2^24 elements apart"""
-    dense = (t.stride(-1) == 1 or t.shape[-1] == 1) and abs(t.stride(token)) < 1 << 24
+    """as the kernels take it: the innermost dimension dense, tokens less than 2^23 elements apart"""
+    dense = (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(token) < 1 << 23
     return t if dense else t.contiguous()
+
+
+def _padding(t):
+    """elements that make a head's dimension whole 16-byte vectors; they are zeros, which no score sees"""
+    return -t.shape[-1] % (4 if t.dtype == torch.float32 else 8)
 
 
 def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=False, key_lengths=None, query_start=0):
     """Attention with ``table[bucket][head]`` added to every score.
 
-    q [batch, heads, m, dim], k / v [batch, kv_heads, n, dim] in fp32, bf16 or fp16, any strides (the innermost dimension is
-    copied if it is not dense); heads a multiple of kv_heads (head h uses key head h // (heads // kv_heads)); dim <= 128.
+    q [batch, heads, m, dim], k / v [batch, kv_heads, n, dim] in fp32, bf16 or fp16, any strides (copied if the innermost
+    dimension is not dense, padded if it is not whole 16-byte vectors); heads a multiple of kv_heads (head h uses key head h // (heads // kv_heads)); dim <= 128.
     table [buckets, heads], fp32, bf16 or fp16.  ``scale`` defaults to dim ** -0.5.
     mask         bool (True: may be seen) or additive, [m, n], [period, m, n] or [period, heads, m, n] with 1 for a dimension it
                  does not depend on; sequence b takes mask b % period (windows of an image).  No gradient.
@@ -316,7 +321,14 @@ def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=Fa
     save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)
     if save and table.requires_grad and o.start_tensor is not None and buckets.distances:
         raise ValueError("the table's gradient needs one query_start for all sequences (an int)")
-    q, k, v, table = _dense_rows(q), _dense_rows(k), _dense_rows(v), table.contiguous()
+    dim, pad = q.shape[3], _padding(q)
+    if pad:
+        q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
+    out = _call(_dense_rows(q), _dense_rows(k), _dense_rows(v), table.contiguous(), o, save)
+    return out[..., :dim] if pad else out
+
+
+def _call(q, k, v, table, o, save):
     if save:
         return _RelativeAttention.apply(q, k, v, table, o)
     out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
@@ -333,5 +345,9 @@ def relative_attention_packed(qkv, table, buckets, scale=None, mask=None, causal
     q = qkv.detach().select(2, 0).transpose(1, 2)
     o = _options(q, q, table, buckets, scale, mask, causal, key_lengths, 0)
     save = torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad)
+    dim, pad = qkv.shape[4], _padding(qkv)
+    if pad:
+        qkv = torch.nn.functional.pad(qkv, (0, pad))
     qkv, table = _dense_rows(qkv, 1), table.contiguous()
-    return _PackedAttention.apply(qkv, table, o) if save else _packed_forward(qkv, table, o, False)[0].flatten(2)
+    out = _PackedAttention.apply(qkv, table, o) if save else _packed_forward(qkv, table, o, False)[0].flatten(2)
+    return out.unflatten(2, (qkv.shape[3], dim + pad))[..., :dim].flatten(2) if pad else out
