@@ -1,5 +1,5 @@
 // Backward of attention with a learned relative position bias.  With p from the forward pass's maximum and sum:
-//     dp_ij = grad_i . v_j      ds_ij = p_ij (dp_ij - delta_i)      delta_i = out_i . grad_i
+//     dp_ij = grad_i . v_j      ds_ij = p_ij (dp_ij - delta_i)      delta_i = sum_j p_ij dp_ij (= out_i . grad_i)
 //     dq_i = scale sum_j ds_ij k_j     dk_j = scale sum_i ds_ij q_i     dv_j = sum_i p_ij grad_i
 //     dtable[u][h] = sum of ds over sequences and over the pairs of bucket u
 // Three kernels in the forward's form, each recomputing the scores: queries stay (dq, and delta for the others), keys stay
@@ -33,6 +33,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
 
     const bool valid = i0 + 16 * wave + c < a.m;
+    const bool busy = wave_any(valid);                   // (a wave behind the last query only stages tiles)
     const int query = min(i0 + 16 * wave + c, a.m - 1);
     const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
     const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
@@ -79,11 +80,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
         if (j0 + ROWS < keys) fetch(j0 + ROWS);
         const Kind kind = tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), true, j0 - pos1 - a.first,
                                             j0 + ROWS - 1 - pos0 - a.first);
-        by_kind<BIASES>(kind, [&](auto tag) {
+        if (busy) by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 s[SUBS], ds[1][SUBS];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             s[t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (decltype(tag)::kind == kEdge && 16 * t >= keys - j0) continue;
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
                 s[t] = mma_row(row_frag<T, DP>(ks, 16 * t + c, dc, g), q[dc], s[t]);
@@ -148,7 +150,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     float* bias_lds = row_delta + 64;
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
-    const int tiles = (a.n + 63) / 64;
     const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.kv_heads) * a.batch;  // as in attention_fwd
     const int hk = static_cast<int>(block % lanes % a.kv_heads);
     const int64_t b = block % lanes / a.kv_heads;
@@ -158,6 +159,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     const bool valid = j0 + 16 * wave + c < a.n;
     const int key = min(j0 + 16 * wave + c, a.n - 1);
     const bool used = valid && key < keys;
+    const bool busy = wave_any(used);
 
     typename Frag<T>::Row k[DC], v[DC];
     const T* kp = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh + static_cast<int64_t>(key) * a.k_sn;
@@ -210,11 +212,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
         const int64_t lead0 = static_cast<int64_t>(j0) - start, lead1 = static_cast<int64_t>(min(j0 + 64, a.n)) - 1 - start;
         const Kind kind = tile_kind<BIASES>(a, i0 + ROWS <= a.m && (!a.causal || i0 >= lead1), true, lead0 - i0 - ROWS + 1 - a.first,
                                             lead1 - i0 - a.first);
-        by_kind<BIASES>(kind, [&](auto tag) {
+        if (busy) by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 p[1][SUBS], ds[1][SUBS];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             p[0][t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (decltype(tag)::kind == kEdge && 16 * t >= a.m - i0) continue;
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
                 p[0][t] = mma_row(row_frag<T, DP>(qs, 16 * t + c, dc, g), k[dc], p[0][t]);
@@ -260,12 +263,13 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int q_tiles = (a.m + 63) / 64, k_tiles = a.distances ? near_tiles(a) : (a.n + 63) / 64;
-    const int64_t block = blockIdx.x;
-    const int k_tile = static_cast<int>(block % k_tiles), q_tile = static_cast<int>(block / k_tiles % q_tiles);
-    const int head = static_cast<int>(block / k_tiles / q_tiles % a.heads);
-    const int chunk = static_cast<int>(block / k_tiles / q_tiles / a.heads);
+    // as in attention_fwd: the tiles of one head and chunk meet in one XCD's L2
+    const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.heads) * a.chunks;
+    const int head = static_cast<int>(block % lanes % a.heads), chunk = static_cast<int>(block % lanes / a.heads);
+    const int k_tile = static_cast<int>(block / lanes % k_tiles), q_tile = static_cast<int>(block / lanes / k_tiles);
     const int i0 = q_tile * 64, j0 = (a.distances ? first_near_tile(a, i0) + k_tile : k_tile) * 64, hk = head / group;
     const bool valid = i0 + 16 * wave + c < a.m;
+    const bool busy = wave_any(valid);
     const int query = min(i0 + 16 * wave + c, a.m - 1);
     if (a.bias_in_lds) stage_bias(a, bias_lds, head, 1, 256);
     f32x4 sum[4];
@@ -273,44 +277,73 @@ __global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
     for (int t = 0; t < 4; ++t) sum[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const int b0 = static_cast<int>(static_cast<int64_t>(a.batch) * chunk / a.chunks);
     const int b1 = static_cast<int>(static_cast<int64_t>(a.batch) * (chunk + 1) / a.chunks);
-    for (int64_t b = b0; b < b1; ++b) {
-        const int start = a.query_start ? a.query_start[b] : a.start;
-        int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
-        if (a.causal) {
-            const int64_t last = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
-            keys = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
+    // the keys that sequence b's queries of this tile see, and the first sequence from b on whose sum this tile takes part in (the same
+    // for the whole workgroup): it has keys in use, and is not past an end of the distances (then it is in attention_bwd_q's sums)
+    auto seen_keys = [&](int64_t b) {
+        const int keys = a.key_lengths ? max(0, min(a.key_lengths[b], a.n)) : a.n;
+        if (!a.causal) return keys;
+        const int64_t last = static_cast<int64_t>(a.query_start ? a.query_start[b] : a.start) + min(i0 + 64, a.m) - 1;
+        return static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(keys), last + 1)));
+    };
+    auto from = [&](int64_t b) {
+        for (; b < b1; ++b) {
+            const int64_t start = a.query_start ? a.query_start[b] : a.start;
+            if (j0 < seen_keys(b) && (a.distances == 0 || far_end(a, j0 - (start + min(i0 + 64, a.m) - 1) - a.first,
+                                                                  j0 + 63 - (start + i0) - a.first) == 0)) break;
         }
-        if (j0 >= keys) continue;                        // (the same for the whole workgroup)
-        if (a.distances && far_end(a, j0 - (static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1) - a.first,
-                                   j0 + 63 - (static_cast<int64_t>(start) + i0) - a.first) != 0) continue;      // in attention_bwd_q's sums
+        return b;
+    };
+    Staged<T, DP, 64, 256> kr, vr;
+    typename Frag<T>::Row next_q[DC], next_go[DC];
+    float next_top = 0.0f, next_inv = 0.0f, next_delta = 0.0f;
+    auto fetch = [&](int64_t b, int keys) {
         const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
         const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
-        Staged<T, DP, 64, 256> kr, vr;
         kr.load(k_base + static_cast<int64_t>(j0) * a.k_sn, a.k_sn, keys - j0, a.dim);
         vr.load(v_base + static_cast<int64_t>(j0) * a.v_sn, a.v_sn, keys - j0, a.dim);
         const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh + query * a.q_sm;
         const T* gp = static_cast<const T*>(a.grad) + b * a.g_sb + head * a.g_sh + query * a.g_sm;
-        typename Frag<T>::Row q[DC], go[DC];
 #pragma unroll
         for (int dc = 0; dc < DC; ++dc) {
-            q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
-            go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
+            next_q[dc] = row_frag_global<T>(qp, a.dim, dc, g, valid);
+            next_go[dc] = row_frag_global<T>(gp, a.dim, dc, g, valid);
         }
         const int64_t at = (b * a.heads + head) * a.m + query;
-        const float top = a.stats[2 * at], inv = valid ? a.stats[2 * at + 1] : 0.0f, delta = a.delta[at];
+        next_top = a.stats[2 * at];
+        next_inv = a.stats[2 * at + 1];
+        next_delta = a.delta[at];
+    };
+    // the next sequence arrives while one is worked on, where registers hold both
+    constexpr bool AHEAD = sizeof(T) == 2 && DP <= 64;
+    int64_t next = from(b0);
+    if (AHEAD && next < b1) fetch(next, seen_keys(next));
+    while (next < b1) {
+        const int64_t b = next;
+        const int start = a.query_start ? a.query_start[b] : a.start, keys = seen_keys(b);
+        if (!AHEAD) fetch(b, keys);
         __syncthreads();
         kr.put(ks);
         vr.put(vs);
+        typename Frag<T>::Row q[DC], go[DC];
+#pragma unroll
+        for (int dc = 0; dc < DC; ++dc) {
+            q[dc] = next_q[dc];
+            go[dc] = next_go[dc];
+        }
+        const float top = next_top, inv = valid ? next_inv : 0.0f, delta = next_delta;
         __syncthreads();
+        next = from(b + 1);
+        if (AHEAD && next < b1) fetch(next, seen_keys(next));
         const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
         const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
         const Kind kind = tile_kind<BIASES>(a, j0 + 64 <= keys && (!a.causal || j0 + 63 <= pos0), true, j0 - pos1 - a.first,
                                             j0 + 63 - pos0 - a.first);
-        by_kind<BIASES>(kind, [&](auto tag) {
+        if (busy) by_kind<BIASES>(kind, [&](auto tag) {
         f32x4 s[4], dp[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             s[t] = dp[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (decltype(tag)::kind == kEdge && 16 * t >= keys - j0) continue;
 #pragma unroll
             for (int dc = 0; dc < DC; ++dc) {
                 s[t] = mma_row(row_frag<T, DP>(ks, 16 * t + c, dc, g), q[dc], s[t]);

@@ -77,6 +77,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 3 : 2) void attent
         m_run[x] = -INFINITY;
         l[x] = 0.0f;
     }
+    const bool busy = wave_any(valid[0]);                // (a wave behind the last query only stages tiles)
     if (keys > 0) {
         kr.put(tiles);
         vr.put(tiles + TILE);
@@ -94,58 +95,61 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 3 : 2) void attent
           do {
             const T* ks = tiles + turn * 2 * TILE;
             const T* vs = ks + TILE;
-            f32x4 s[NQ][SUBS];
+            if (busy) {
+                f32x4 s[NQ][SUBS];
 #pragma unroll
-            for (int t = 0; t < SUBS; ++t) {
+                for (int t = 0; t < SUBS; ++t) {
 #pragma unroll
-                for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int x = 0; x < NQ; ++x) s[x][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (decltype(tag)::kind == kEdge && 16 * t >= keys - j0) continue;
 #pragma unroll
-                for (int dc = 0; dc < DC; ++dc) {
-                    const typename Frag<T>::Row kf = row_frag<T, DP>(ks, 16 * t + c, dc, g);
+                    for (int dc = 0; dc < DC; ++dc) {
+                        const typename Frag<T>::Row kf = row_frag<T, DP>(ks, 16 * t + c, dc, g);
 #pragma unroll
-                    for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
+                        for (int x = 0; x < NQ; ++x) s[x][t] = mma_row(kf, q[x][dc], s[x][t]);
+                    }
                 }
-            }
-            bool more = false;
-            float top[NQ];
-#pragma unroll
-            for (int x = 0; x < NQ; ++x) {
-                score_tile<BIASES, decltype(tag)::kind, false>(a, col[x], j0, g, s[x]);
-                top[x] = s[x][0][0];
-#pragma unroll
-                for (int t = 0; t < SUBS; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) top[x] = fmaxf(top[x], s[x][t][r]);
-                top[x] = reduce_rows(top[x], [](float u, float v) { return fmaxf(u, v); });
-                more = more || top[x] > m_run[x] + kSlack;
-            }
-            // The reference is the largest score up to 2^kSlack: sums and outputs are rescaled only where one exceeds it by
-            // more, which after a few tiles is hardly ever.  (Probabilities up to 2^kSlack cost no precision.)
-            if (__ballot(more) != 0) {
+                bool more = false;
+                float top[NQ];
 #pragma unroll
                 for (int x = 0; x < NQ; ++x) {
-                    const float m_new = fmaxf(m_run[x], top[x]);
-                    const float shrink = m_new == -INFINITY ? 1.0f : exp2_hw(m_run[x] - m_new);
-                    m_run[x] = m_new;
-                    l[x] *= shrink;
+                    score_tile<BIASES, decltype(tag)::kind, false>(a, col[x], j0, g, s[x]);
+                    top[x] = s[x][0][0];
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
+                    for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) top[x] = fmaxf(top[x], s[x][t][r]);
+                    top[x] = reduce_rows(top[x], [](float u, float v) { return fmaxf(u, v); });
+                    more = more || top[x] > m_run[x] + kSlack;
                 }
-            }
+                // The reference is the largest score up to 2^kSlack: sums and outputs are rescaled only where one exceeds it by
+                // more, which after a few tiles is hardly ever.  (Probabilities up to 2^kSlack cost no precision.)
+                if (__ballot(more) != 0) {
 #pragma unroll
-            for (int x = 0; x < NQ; ++x) {
-                const float m_ref = m_run[x] == -INFINITY ? 0.0f : m_run[x];
-                float sum = 0.0f;
+                    for (int x = 0; x < NQ; ++x) {
+                        const float m_new = fmaxf(m_run[x], top[x]);
+                        const float shrink = m_new == -INFINITY ? 1.0f : exp2_hw(m_run[x] - m_new);
+                        m_run[x] = m_new;
+                        l[x] *= shrink;
 #pragma unroll
-                for (int t = 0; t < SUBS; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        s[x][t][r] = exp2_hw(s[x][t][r] - m_ref);
-                        sum += s[x][t][r];
+                        for (int dt = 0; dt < DT; ++dt) o[x][dt] *= shrink;
                     }
-                l[x] += sum;
+                }
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) {
+                    const float m_ref = m_run[x] == -INFINITY ? 0.0f : m_run[x];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            s[x][t][r] = exp2_hw(s[x][t][r] - m_ref);
+                            sum += s[x][t][r];
+                        }
+                    l[x] += sum;
+                }
+                mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
             }
-            mma_transposed<DP, NQ, SUBS>(vs, s, o, c, g);
             if (j0 + ROWS < keys) {
                 T* next = tiles + (turn ^ 1) * 2 * TILE; // (everyone has left it: the barrier of the last turn)
                 kr.put(next);

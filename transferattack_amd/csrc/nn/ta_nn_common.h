@@ -110,6 +110,7 @@ struct Max {                                             // NaN wins
     __device__ __forceinline__ float operator()(float a, float b) const { return max_nan(a, b); }
     __device__ __forceinline__ double operator()(double a, double b) const { return (a > b || a != a) ? a : b; }
 };
+__device__ __forceinline__ bool wave_any(bool v) { return __ballot(v) != 0; }
 template <class V> __device__ __forceinline__ V wave_sum(V v) { return reduce_wave(v, Sum{}); }
 template <class V> __device__ __forceinline__ V wave_max(V v) { return reduce_wave(v, Max{}); }
 // `lds`: one V per wave; the barriers make it free for the next call
