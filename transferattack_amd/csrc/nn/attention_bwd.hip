@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
 // ds of one tile of 64 queries x 64 keys of a head, summed over the sequences of a chunk.  Pairs: the tile as it is; distances:
 // its 127 diagonals (the distance is the same along each), and only tiles that are not past an end altogether.
 template <class T, int DP, int BIASES>
-__global__ __launch_bounds__(256, 2) void attention_bwd_table(AttentionArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_table(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);

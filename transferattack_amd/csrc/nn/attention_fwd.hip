@@ -184,15 +184,22 @@ template <class T, int DP, int NQ> int launch_forward_by(AttentionArgs a, hipStr
     const int64_t blocks = tiles * a.kv_heads * a.batch;
     TA_NN_REQUIRE(blocks <= 0x7FFFFFFF, "too many queries: %lld workgroups", static_cast<long long>(blocks));
     const size_t lds = 4 * 16 * kSubs<DP> * Tile<T, DP>::LD * sizeof(T) + bias_lds_bytes(a, 64 * NQ);
-    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_fwd<T, DP, NQ, BIASES>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a));
+    if constexpr (NQ == 2) {                             // pairs only: no instance for distances
+        if (biases_of(a) == kByPair) hipLaunchKernelGGL((attention_fwd<T, DP, NQ, kByPair>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
+        else hipLaunchKernelGGL((attention_fwd<T, DP, NQ, kAny>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a);
+    } else {
+        TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_fwd<T, DP, NQ, BIASES>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds, st, a));
+    }
     return check_launch("ta_nn_attention");
 }
 
 template <class T, int DP> int launch_forward(AttentionArgs a, hipStream_t st) {
     const int64_t columns = static_cast<int64_t>(a.heads / a.kv_heads) * a.m;
-    // 32 columns to a wave halve the LDS reads per product, which is what 16-bit products wait for; not where that leaves CUs idle,
-    // nor for wide heads, whose accumulators then leave room for two waves to a SIMD only
-    if (sizeof(T) == 2 && DP <= 64 && ceil_div(columns, 128) * a.kv_heads * a.batch >= 512) return launch_forward_by<T, DP, sizeof(T) == 2 && DP <= 64 ? 2 : 1>(a, st);
+    // 32 columns to a wave halve the LDS reads per product, but leave room for two waves to a SIMD instead of three: 48 against 53 us
+    // for pairs (64 x 12 heads, 196 tokens of 64, bf16), 63 against 57 us for distances (8 x 12 heads, 1023 tokens of 64), whose
+    // scores are ready sooner.  Not where it leaves CUs idle, nor for wide heads, whose accumulators leave no room.
+    constexpr int WIDE = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+    if (WIDE == 2 && a.distances == 0 && ceil_div(columns, 128) * a.kv_heads * a.batch >= 512) return launch_forward_by<T, DP, WIDE>(a, st);
     return launch_forward_by<T, DP, 1>(a, st);
 }
 
