@@ -338,6 +338,36 @@ def check_differences(device):
     assert abs(float((grad * d).sum()) - float(f[0] - f[1]) / (2 * h)) <= float((bound * d.abs()).sum()) + 1e-7
 
 
+def check_few_keys(dtype, device):
+    """two keys whose values are neighbours in `dtype`: dp_j - sum p dp is of the order of one step of the values, so dq's kernel must
+    not take that sum from the rounded output.  With t half a step of dtype and U of fp32: ds is off by t |ds| from its rounding, by
+    p 2 rel |dp_0 - dp_1| from probabilities off by rel = 2 (dim + 4) U size + 16 U each, and by p 2 (dim + 8) U |grad| . |v| from dp and
+    its sum; dq by those over |k|, and by t |dq| from its own rounding."""
+    gen = torch.Generator().manual_seed(11)
+    m, dim, U, t = 70, 32, 2.0 ** -24, nn_oracle.half_step(dtype)
+    q, grad = (torch.randn(2, 3, m, dim, generator=gen).to(dtype) for _ in range(2))
+    k = torch.randn(2, 3, 2, dim, generator=gen).to(dtype)
+    first = torch.rand(2, 3, 1, dim, generator=gen).add(1.0).to(dtype)
+    v = torch.cat([first, (first.float() + 2 * t).to(dtype)], 2)          # in [1, 2): the next value
+    table = torch.randn(4, 3, generator=gen)
+    index = torch.randint(0, 4, (m, 2), generator=gen)
+    leaves = [x.to(device).requires_grad_(True) for x in (q, k, v)]
+    out = relative_attention(*leaves, table.to(device), RelativeBuckets.from_index(index.to(device)))
+    (dq,) = torch.autograd.grad(out, leaves[:1], grad.to(device))
+    q, k, v, grad = (x.double() for x in (q, k, v, grad))
+    scale = dim ** -0.5
+    bias = table.double()[index].movedim(-1, 0)
+    size = (q.abs() @ k.abs().transpose(-2, -1) * scale + bias.abs()).amax(-1, keepdim=True)
+    p = (q @ k.transpose(-2, -1) * scale + bias).softmax(-1)
+    dp = grad @ v.transpose(-2, -1)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    rel = 2 * (dim + 4) * U * size + 16 * U
+    apart = (dp[..., :1] - dp[..., 1:]).abs()
+    off = t * ds.abs() + p * (2 * rel * apart + 2 * (dim + 8) * U * (grad.abs() @ v.abs().transpose(-2, -1)).amax(-1, keepdim=True))
+    want = ds @ k * scale
+    assert ((dq.cpu().double() - want).abs() <= 1.01 * (off @ k.abs() * scale + t * want.abs())).all()
+
+
 def check_broadcast_inputs(device):
     """inputs expanded over the batch (stride 0): read as they are, their gradients summed by autograd"""
     gen = torch.Generator().manual_seed(1)

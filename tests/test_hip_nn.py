@@ -75,6 +75,11 @@ def test_gradients_against_differences():
     cases.check_differences(DEV)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_few_keys(dtype):
+    cases.check_few_keys(dtype, DEV)
+
+
 def test_broadcast_inputs():
     cases.check_broadcast_inputs(DEV)
 

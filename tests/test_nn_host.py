@@ -56,6 +56,11 @@ def test_gradients_against_differences(host):
     cases.check_differences("cpu")
 
 
+@pytest.mark.parametrize("dtype", [cases.BF16, cases.F16])
+def test_few_keys(host, dtype):
+    cases.check_few_keys(dtype, "cpu")
+
+
 def test_broadcast_inputs(host):
     cases.check_broadcast_inputs("cpu")
 

@@ -15,7 +15,7 @@ namespace ta_nn {
 
 struct AttentionArgs : ta_nn_attention_args {
     int bias_in_lds;                                     // the bias values of a block's heads are staged in LDS
-    float* delta;                                        // [batch][heads][m]: sum_d out grad
+    float* delta;                                        // [batch][heads][m]: sum_j p dp
     float* partial;                                      // sums of score gradients, per batch chunk
     float* far;                                          // distances: [batch][heads][64 queries][2] sums past either end
     float* by_distance;                                  // distances: [heads][64 (tile difference)][128] sums of the near tiles

@@ -5,6 +5,11 @@
 // Three kernels in the forward's form, each recomputing the scores: queries stay (dq, and delta for the others), keys stay
 // (dk, dv), and a tile of pairs stays while the batch streams past it (the table).  No sum crosses workgroups except the
 // table's, whose partial sums a last kernel adds in a fixed order.
+// Together 9 products of m n dim, the forward's two aside, where 5 are needed: scores and dp are computed once for each kernel
+// rather than 16-bit sums exchanged through atomics, whose order would change results.  Bound like the forward by LDS reads and
+// issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 74 us, keys 87, table 42 + 20 (near tiles only: what is
+// past an end of the distances is summed by the queries' kernel, which meets those pairs anyway); 64 x 12 x 196 tokens in pairs,
+// 50, 57, 59 + 15 us.  64-row tiles (two waves to a SIMD) instead of 32: 81 and 105 us for the first two.
 #include "attention.h"
 
 namespace ta_nn {
@@ -57,6 +62,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
 
     // delta for this kernel is out . grad.  For 16-bit tensors out is rounded, and so were the probabilities it was made with; for
     // the table, whose gradient is a sum of differences that nearly cancel, and for the keys it is taken anew: sum_j p_ij dp_ij.
+    // So it is for this kernel where a row is a single tile: with few keys out is as large as they are, and its rounding counts
+    // (over n keys it weighs a sqrt(n)-th of that of ds).
     float exact = 0.0f;
     // sums past either end of the distances, for the table: of p and of p dp, since delta is not known yet
     float far_p[2] = {0.0f, 0.0f}, far_dp[2] = {0.0f, 0.0f};
@@ -98,11 +105,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = exp2_hw(s[t][r] - top) * inv, dp = ds[0][t][r];
-                ds[0][t][r] = p * (dp - delta);
-                s[t][r] = p;
-                exact_tile += p * dp;
+                s[t][r] = exp2_hw(s[t][r] - top) * inv;
+                exact_tile += s[t][r] * ds[0][t][r];
             }
+        if (keys <= ROWS) delta = reduce_rows(exact_tile, Sum{});
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ds[0][t][r] = s[t][r] * (ds[0][t][r] - delta);
         exact += exact_tile;
         if constexpr (BIASES != kByPair && decltype(tag)::kind != kNear) {
             const int64_t j64 = j0 & ~63;
@@ -263,7 +273,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const int group = a.heads / a.kv_heads;
     const int q_tiles = (a.m + 63) / 64, k_tiles = a.distances ? near_tiles(a) : (a.n + 63) / 64;
-    // as in attention_fwd: the tiles of one head and chunk meet in one XCD's L2
+    // as in attention_fwd: the tiles of one head and chunk meet in one XCD's L2 (tile by tile over all of them: 67 us, so: 52)
     const int64_t block = blockIdx.x, lanes = static_cast<int64_t>(a.heads) * a.chunks;
     const int head = static_cast<int>(block % lanes % a.heads), chunk = static_cast<int>(block % lanes / a.heads);
     const int k_tile = static_cast<int>(block / lanes % k_tiles), q_tile = static_cast<int>(block / lanes / k_tiles);

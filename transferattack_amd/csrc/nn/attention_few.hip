@@ -2,7 +2,9 @@
 // the next token of every sequence meets its cache.  Bound by reading keys and values once, so nothing is shared between waves:
 // each takes 32 keys (wide fp32 heads: 16) at a time for itself, keys straight from memory into the matrix instruction's layout, values through
 // as many rows of LDS of its own, with its own maximum and sum; the next ones are on their way while it works.  A workgroup's four
-// waves are joined in LDS, the workgroups of a long sequence by a second kernel.
+// waves are joined in LDS, the workgroups of a long sequence by a second kernel.  Measured: 32 sequences of up to 16384 keys, 4 key
+// heads of 128 in bf16, 142 us (4.7 TB/s; a large copy reaches 5.0) and 7 us for the join; 1 x 12 heads x 511 keys of 64, 8 us, of
+// which the launch is most.  With waves sharing tiles through LDS and a barrier for each the first took 1880 us.
 #include "attention.h"
 
 namespace ta_nn {

@@ -3,7 +3,9 @@
 // registers (16 to a lane), and streams sequences of its head past them: the next arrives in registers while one is worked on.
 // Backward computes everything of a sequence at once, scores once instead of once per gradient: probabilities and score
 // gradients are transposed through LDS for dk and dv, and score gradients add up in registers over the workgroup's sequences
-// for the table.  What bounds it: fp32 products (7 of 64 x 64 x dim a sequence at a 16th of the 16-bit rate) and memory alike.
+// for the table.  What bounds it: fp32 products (7 of 64 x 64 x dim a sequence, a tenth of the 16-bit rate, 49 of 64 rows and
+// columns in use) and memory alike: 8000 windows x 3 heads of 49 x 32 in fp32 with a mask for each of 64 windows, forward 147 us
+// (3.3 TB/s), backward 375 us (2.1 TB/s of q, k, v, gradients and output; matrix units half busy); 32 x 24 without mask, 12.5 us.
 #include "attention.h"
 
 namespace ta_nn {

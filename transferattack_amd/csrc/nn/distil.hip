@@ -197,6 +197,8 @@ __device__ __forceinline__ void top_gradients(const DistilArgs& a, int64_t row, 
 // The vector units are what limits this: with 32 000 classes there is time for some 25 operations an element at the memory's
 // rate, an exponential being four.  So the classes answered are set to -inf where the row lies in registers, once, instead of
 // being asked for in every pass; the exponentials take their place there (as far as there is room) and the gradient is a product.
+// Measured: loss and gradient of 8192 x 32768 bf16 against 32 classes, 243 us (4.4 TB/s; a large copy reaches 5.0); statistics of
+// 4095 x 21841 fp32 against 17, 134 us (2.7 TB/s).
 template <class T, int THREADS, int VPT, bool GRAD>
 __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
     constexpr int WAVES = THREADS / 64, N = Vec<T>::N;
@@ -352,7 +354,8 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
     }
 }
 
-// The gradient from the statistics of the forward pass: one read and one write of the row.
+// The gradient from the statistics of the forward pass: one read and one write of the row.  4095 x 21841 fp32, 110 us (6.5 TB/s, part
+// of the row still in the cache that the forward pass left).
 template <class T, int THREADS>
 __global__ __launch_bounds__(THREADS) void distil_backward(DistilArgs a) {
     constexpr int N = Vec<T>::N;
@@ -448,6 +451,8 @@ __device__ __forceinline__ float value_of_order(unsigned o) {          // the in
 // bisection over its 64 bits, reading the row again for each.
 // In the common case an element is looked at twice in registers: for its vector's maximum and for its exponential.  Vectors that
 // reach the limit, one or two for each of the K, are copied to LDS and leave the row; their elements get a thread each.
+// Measured: 64 of 65536 bf16, 4096 rows, 170 us (3.1 TB/s: vector units and the first wave's ranking, several rows to a CU at
+// different stages); 5 of 1000 fp32, 32 rows, 5.6 us, most of it the launch and one row's chain of dependent steps.
 template <class T, int THREADS, int VPT>
 __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {
     constexpr int WAVES = THREADS / 64, N = Vec<T>::N, KEPT = VPT > 0 ? VPT : 1;
