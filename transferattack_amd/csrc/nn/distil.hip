@@ -198,7 +198,7 @@ __device__ __forceinline__ void top_gradients(const DistilArgs& a, int64_t row, 
 // rate, an exponential being four.  So the classes answered are set to -inf where the row lies in registers, once, instead of
 // being asked for in every pass; the exponentials take their place there (as far as there is room) and the gradient is a product.
 // Measured: loss and gradient of 8192 x 32768 bf16 against 32 classes, 243 us (4.4 TB/s; a large copy reaches 5.0); statistics of
-// 4095 x 21841 fp32 against 17, 134 us (2.7 TB/s).
+// 4095 x 21841 fp32 against 17, 123 us (2.9 TB/s).
 template <class T, int THREADS, int VPT, bool GRAD>
 __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
     constexpr int WAVES = THREADS / 64, N = Vec<T>::N;
@@ -682,6 +682,7 @@ template <class T, bool GRAD> int launch_rows(const DistilArgs& a, int64_t rows,
     if (vectors <= 64 * 4) hipLaunchKernelGGL((distil_rows<T, 64, 4, GRAD>), grid, dim3(64), lds, st, a);
     else if (vectors <= 256 * 4) hipLaunchKernelGGL((distil_rows<T, 256, 4, GRAD>), grid, dim3(256), lds, st, a);
     else if (vectors <= 256 * 16) hipLaunchKernelGGL((distil_rows<T, 256, 16, GRAD>), grid, dim3(256), lds, st, a);
+    else if (vectors <= 512 * 12) hipLaunchKernelGGL((distil_rows<T, 512, 12, GRAD>), grid, dim3(512), lds, st, a);     // 21841 fp32: 123 us (16: 135)
     else if (vectors <= 512 * 16) hipLaunchKernelGGL((distil_rows<T, 512, 16, GRAD>), grid, dim3(512), lds, st, a);
     else hipLaunchKernelGGL((distil_rows<T, 1024, 0, GRAD>), grid, dim3(1024), lds, st, a);
     return check_launch("ta_nn_distil");
