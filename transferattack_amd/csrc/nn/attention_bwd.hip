@@ -5,6 +5,8 @@
 // Three kernels in the forward's form, each recomputing the scores: queries stay (dq, and delta for the others), keys stay
 // (dk, dv), and a tile of pairs stays while the batch streams past it (the table).  No sum crosses workgroups except the
 // table's, whose partial sums a last kernel adds in a fixed order.
+// p and ds are rounded to 16 bits where they enter a 16-bit matrix instruction: half a step of each term.  In fp16 terms below 2^-14
+// keep 2^-25 absolutely (p over more than some 10 000 equal keys, gradients below 6e-5: the same that their results are rounded by).
 // Together 9 products of m n dim, the forward's two aside, where 5 are needed: scores and dp are computed once for each kernel
 // rather than 16-bit sums exchanged through atomics, whose order would change results.  Bound like the forward by LDS reads and
 // issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 74 us, keys 87, table 42 + 20 (near tiles only: what is
