@@ -243,6 +243,7 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
     if (tid < 64) {
         const TopSide t = top_side(a, row, cls, x, repeats);
         if (tid == 0) side = t;
+        wave_lds_order();                                // only this wave reads it, in workgroups of one wave without a barrier between
     }
     const unsigned char* mark_bytes = reinterpret_cast<const unsigned char*>(smem);
     auto unmarked = [&](int j, Vec<T> v) -> Vec<T> {     // the classes answered are not among the others
