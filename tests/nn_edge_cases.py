@@ -1,0 +1,73 @@
+"""Calls of the operators in transferattack_amd.relative / .distill that nn_cases does not make, shared by the host tier and the GPU
+tier: the same functions, the device given by the caller.
+
+Bounds are counted as in nn_oracle: u = 2^-24 is half a step of fp32, t half a step of the tensors' type."""
+import torch
+
+import nn_oracle
+from nn_cases import BF16, F16, F32  # noqa: F401
+from transferattack_amd.distill import TopLogits, distillation_loss, distillation_loss_and_grad, top_logits
+
+U = nn_oracle.U
+
+
+def distil_rows_64(x, values, classes, rest, temperature):
+    """-> loss [rows] and its gradient [rows, n] in 64 bits, from logarithms throughout (a share of a mass that underflows is kept), and
+    what bounds them: w [rows, n], every other class's share of the others, and log q_R"""
+    x, values = x.detach().cpu().double() / temperature, values.detach().cpu().double() / temperature
+    bins = values if rest is None else torch.cat([values, rest.detach().cpu().double()[:, None]], 1)
+    log_p = torch.log_softmax(bins, 1)
+    log_q = torch.log_softmax(x, 1)
+    answered = torch.zeros_like(x, dtype=torch.bool).scatter_(1, classes.cpu(), True)
+    log_rest = log_q.masked_fill(answered, -torch.inf).logsumexp(1, keepdim=True)
+    at = log_q.gather(1, classes.cpu())
+    w = torch.softmax(x.masked_fill(answered, -torch.inf), 1)      # (log_q - log_rest would lose log n beside a masking constant)
+    p = log_p.exp()
+    p_rest = torch.zeros_like(log_rest)
+    if rest is not None:
+        at, p_rest = torch.cat([at, log_rest], 1), p[:, -1:]
+    loss = temperature ** 2 * torch.where(p > 0, p * (log_p - at), torch.zeros_like(p)).sum(1)
+    grad = log_q.exp() - w * p_rest
+    grad.scatter_add_(1, classes.cpu(), -p[:, :classes.shape[1]])
+    return loss, temperature * grad, w, log_rest, p_rest
+
+
+def check_masked_rest(dtype, masked, temperature, device):
+    """a teacher whose classes but six are ruled out by a constant: the answers take those six and two of the others, and what is left is
+    the constant's: log 290 + masked / T.  The logarithm of a sum of 290 exponentials of 0, whose error is 2 u of each, and the
+    result's rounding, u"""
+    gen = torch.Generator().manual_seed(0)
+    x = torch.full((3, 298), masked, dtype=torch.float64).to(dtype)
+    x[:, 5:11] = torch.randn(3, 6, generator=gen).to(dtype)
+    got = top_logits(x.to(device), 8, temperature=temperature)
+    want = x[0, 0].double() / temperature + torch.tensor(290.0).double().log()
+    assert torch.equal(got.classes.cpu()[:, 6:], torch.tensor([[0, 1]]).expand(3, 2))
+    assert ((got.rest.cpu().double() - want).abs() <= 4 * U + U * want.abs()).all(), (got.rest, want)
+
+
+def check_masked_student(dtype, masked, temperature, rest, device):
+    """a student that rules out every class not answered by a constant, in both forms.  The sum of the others (292 exponentials of 0) is
+    off by 4 u at most, and so is each one's share; what concerns the answers is 64-bit, and rounded to 32 bits once or twice"""
+    gen = torch.Generator().manual_seed(1)
+    rows, n, top = 3, 300, 8
+    x = torch.full((rows, n), masked, dtype=torch.float64).to(dtype)
+    classes = torch.stack([torch.randperm(n, generator=gen)[:top] for _ in range(rows)])
+    x.scatter_(1, classes, torch.randn(rows, top, generator=gen).to(dtype))
+    values = torch.randn(rows, top, generator=gen)
+    left = torch.full((rows,), -3.0) if rest else None
+    loss, grad, w, log_rest, p_rest = distil_rows_64(x, values, classes, left, temperature)
+    answers = TopLogits(values.to(device), classes.to(device), None if left is None else left.to(device), temperature)
+    xx = x.to(device).requires_grad_(True)
+    got = distillation_loss(xx, answers, reduction="sum")
+    (dx,) = torch.autograd.grad(got, xx)
+    both = distillation_loss_and_grad(xx, answers, reduction="sum")
+    t = nn_oracle.half_step(dtype)
+    # a class answered: q off by 2 u (1 / Z kept in 32 bits); any other: its share by 8 u, and the smallest number of the type
+    off = temperature * (2 * U + 8 * U * w * p_rest) + (t + 2 * U) * grad.abs() + float(torch.finfo(dtype).smallest_normal) * 2 * t
+    for l, g in ((got, dx), both):
+        assert abs(float(l.detach()) - float(loss.sum())) <= 8 * U * float(loss.abs().sum()) + 8 * U * temperature ** 2, (float(l.detach()), float(loss.sum()))
+        assert ((g.cpu().double() - grad).abs() <= off).all(), (g.cpu().double() - grad).abs().max()
+
+
+MASKING = [(F32, -1e10), (F32, -1e20), (F32, -1e30), (F32, torch.finfo(F32).min), (BF16, -1e10), (BF16, torch.finfo(BF16).min),
+           (F16, torch.finfo(F16).min)]

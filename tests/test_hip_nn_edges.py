@@ -1,0 +1,20 @@
+"""nn_edge_cases on the GPU (libta_nn.so)."""
+import pytest
+
+import nn_edge_cases as edges
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("dtype,masked", edges.MASKING)
+def test_masked_rest(dtype, masked, temperature):
+    edges.check_masked_rest(dtype, masked, temperature, DEV)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("dtype,masked", edges.MASKING)
+def test_masked_student(dtype, masked, temperature, rest):
+    edges.check_masked_student(dtype, masked, temperature, rest, DEV)

@@ -1,0 +1,27 @@
+"""nn_edge_cases where there is no GPU: the kernel sources compiled for the host, driven through the package's binding."""
+import os
+import sys
+
+import pytest
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "hipcpu_nn"))
+import nn_edge_cases as edges        # noqa: E402
+import nn_host_build                 # noqa: E402
+
+
+@pytest.fixture
+def host(monkeypatch):
+    nn_host_build.install(monkeypatch)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("dtype,masked", edges.MASKING)
+def test_masked_rest(host, dtype, masked, temperature):
+    edges.check_masked_rest(dtype, masked, temperature, "cpu")
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+@pytest.mark.parametrize("dtype,masked", edges.MASKING)
+def test_masked_student(host, dtype, masked, temperature, rest):
+    edges.check_masked_student(dtype, masked, temperature, rest, "cpu")

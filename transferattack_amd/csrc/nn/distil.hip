@@ -39,7 +39,7 @@ struct DistilArgs {
     int64_t grad_stride;
 };
 
-constexpr int kStats = 5;                                // d, (q_R - p_R) / s, M = max over all, 1 / Z, whether a class repeats
+constexpr int kStats = 5;                                // m, (q_R - p_R) / s, M = max over all, 1 / Z, whether a class repeats
 
 __device__ __forceinline__ int class_at(const DistilArgs& a, int64_t row, int i) {
     const int64_t at = row * a.k + i;
@@ -271,11 +271,11 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
     }
     r.forget_unpacked();
     m = block_max<WAVES>(m, red_f);
-    // exponentials are taken as 2^(x c - d): one product-sum.  d is the rounded m c; what it is off by is the same for the
-    // whole row, and is put back, in 64 bits, where s meets the classes answered.
+    // exponentials are taken as 2^((x - m) c), the difference first: 2^(x c - m c) would be one product-sum, but the rounding of m c
+    // is as large as the exponent itself where every other class holds a masking constant (-1e10 and below)
     const float c2 = static_cast<float>(1.4426950408889634 / a.temperature);
-    const float d = (m == -INFINITY ? 0.0f : m) * c2;
-    r.tail = exp2_hw(fmaf(r.tail, c2, -d));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    r.tail = exp2_hw((r.tail - ref) * c2);
     float part = r.tail;
     float kept[KEEP ? VPT : 1][N];
 #pragma unroll VPT > 0 ? VPT : 1
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float e = exp2_hw(fmaf(get(v, i), c2, -d));
+            const float e = exp2_hw((get(v, i) - ref) * c2);
             sum += e;
             if constexpr (KEEP) kept[j][i] = e;
         }
@@ -303,10 +303,8 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
         const double per_t = 1.0 / a.temperature;
         m_all = (m > t.x_max || t.x_max != t.x_max) ? static_cast<double>(m) : t.x_max;
         if (t.x_max != t.x_max) m_all = t.x_max;
-        // s is relative to 2^d: to exp(m_all / T) instead
-        const double ln2 = 0.6931471805599453;
-        const double shift = m == -INFINITY ? -INFINITY : (static_cast<double>(d) - static_cast<double>(m) * static_cast<double>(c2)) * ln2
-                                                              + (static_cast<double>(m) - m_all) * per_t;
+        // s is relative to exp(m / T): to exp(m_all / T) instead
+        const double shift = m == -INFINITY ? -INFINITY : (static_cast<double>(m) - m_all) * per_t;
         const double others = s == 0.0 ? 0.0 : s * exp(shift);
         double z = others + (t.x_sum == 0.0 ? 0.0 : t.x_sum * exp((t.x_max - m_all) * per_t));
         if (m_all == -INFINITY) z = NAN;                 // no class has any weight: not a distribution
@@ -322,7 +320,7 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
         if (tid == 0) {
             a.row_loss[row] = static_cast<float>(kl * a.temperature * a.temperature * static_cast<double>(w));
             if (stats) {
-                stats[0] = d;
+                stats[0] = ref;
                 stats[1] = static_cast<float>(kappa);
                 stats[2] = static_cast<float>(m_all);
                 stats[3] = static_cast<float>(inv_z);
@@ -344,7 +342,7 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
             for (int i = 0; i < N; ++i) {
                 float e;
                 if constexpr (KEEP) e = kept[j][i];
-                else e = exp2_hw(fmaf(get(v, i), c2, -d));
+                else e = exp2_hw((get(v, i) - ref) * c2);
                 o[i] = e * each;
             }
             store_vec(grad + at, pack<T>(o));
@@ -371,7 +369,7 @@ __global__ __launch_bounds__(THREADS) void distil_backward(DistilArgs a) {
         return;
     }
     const float* stats = a.stats + row * kStats;
-    const float d = stats[0], kappa = stats[1], m_all = stats[2], inv_z = stats[3];
+    const float ref = stats[0], kappa = stats[1], m_all = stats[2], inv_z = stats[3];
     const bool repeats = stats[4] != 0.0f;
     double coef = a.temperature * static_cast<double>(w) * static_cast<double>(a.factor);
     if (a.scale) coef *= static_cast<double>(*a.scale);
@@ -388,10 +386,10 @@ __global__ __launch_bounds__(THREADS) void distil_backward(DistilArgs a) {
         const Vec<T> v = load_vec(x + at);
         float o[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = exp2_hw(fmaf(get(v, i), c2, -d)) * each;
+        for (int i = 0; i < N; ++i) o[i] = exp2_hw((get(v, i) - ref) * c2) * each;
         store_vec(grad + at, pack<T>(o));
     }
-    if (full + tid < a.classes) grad[full + tid] = from_float<T>(exp2_hw(fmaf(to_float(x[full + tid]), c2, -d)) * each);
+    if (full + tid < a.classes) grad[full + tid] = from_float<T>(exp2_hw((to_float(x[full + tid]) - ref) * c2) * each);
     __syncthreads();
     if (tid < 64 && inv_z == inv_z && kappa == kappa) {
         const TopSide t = top_side(a, row, cls, x, repeats);
@@ -646,12 +644,12 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {
     r.forget_unpacked();
     m = block_max<WAVES>(m, red_f);
     const float c2 = static_cast<float>(1.4426950408889634 / static_cast<double>(a.temperature));
-    const float d = (m == -INFINITY ? 0.0f : m) * c2;    // as in distil_rows
-    float part = exp2_hw(fmaf(r.tail, c2, -d));
+    const float ref = m == -INFINITY ? 0.0f : m;         // as in distil_rows
+    float part = exp2_hw((r.tail - ref) * c2);
     auto add = [&](const Vec<T>& v) {
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum += exp2_hw(fmaf(get(v, i), c2, -d));
+        for (int i = 0; i < N; ++i) sum += exp2_hw((get(v, i) - ref) * c2);
         part += sum;
     };
     if (kept) {
@@ -659,7 +657,7 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {
         for (int j = 0; j < KEPT; ++j) add(r.kept[j]);
         for (int e = tid; e < pairs; e += THREADS) {
             const float f = element_of(e);
-            if (key_of(f, hit_at[e / N] + e % N) < last) part += exp2_hw(fmaf(f, c2, -d));
+            if (key_of(f, hit_at[e / N] + e % N) < last) part += exp2_hw((f - ref) * c2);
         }
     } else {
 #pragma unroll 1
@@ -667,8 +665,7 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {
     }
     const double s = block_sum<WAVES>(static_cast<double>(part), red_d);
     if (tid == 0) {
-        const double off = static_cast<double>(d) - (m == -INFINITY ? 0.0 : static_cast<double>(m) * static_cast<double>(c2));
-        const double value = static_cast<double>(m) / static_cast<double>(a.temperature) + off * 0.6931471805599453 + log(s);
+        const double value = static_cast<double>(m) / static_cast<double>(a.temperature) + log(s);
         a.rest[row] = m == -INFINITY || m == INFINITY ? m : static_cast<float>(value);
     }
 }
