@@ -71,3 +71,19 @@ def check_masked_student(dtype, masked, temperature, rest, device):
 
 MASKING = [(F32, -1e10), (F32, -1e20), (F32, -1e30), (F32, torch.finfo(F32).min), (BF16, -1e10), (BF16, torch.finfo(BF16).min),
            (F16, torch.finfo(F16).min)]
+
+
+def check_top_repeats(rows, classes, top, dtype, device, turns=12):
+    """the same answers, to the bit, whatever ran before and in whatever order a row's waves came"""
+    gen = torch.Generator().manual_seed(2)
+    x = (torch.randn(rows, classes, generator=gen) * 3).to(dtype).to(device)
+    first = top_logits(x, top, temperature=2.0)
+    want = nn_oracle.top_logits(x, top, 2.0, dtype)[2]
+    assert ((first.rest.cpu().double() - want[0]).abs() <= want[1]).all()
+    for _ in range(turns):
+        got = top_logits(x, top, temperature=2.0)
+        assert torch.equal(got.values, first.values) and torch.equal(got.classes, first.classes)
+        assert torch.equal(got.rest, first.rest), int((got.rest != first.rest).sum())
+
+
+REPEATED = [(2351, 1541, 55, F32), (325, 4721, 11, BF16), (900, 1000, 64, F32), (700, 30000, 40, F16)]

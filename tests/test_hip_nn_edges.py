@@ -18,3 +18,8 @@ def test_masked_rest(dtype, masked, temperature):
 @pytest.mark.parametrize("dtype,masked", edges.MASKING)
 def test_masked_student(dtype, masked, temperature, rest):
     edges.check_masked_student(dtype, masked, temperature, rest, DEV)
+
+
+@pytest.mark.parametrize("rows,classes,top,dtype", edges.REPEATED)
+def test_top_logits_repeat(rows, classes, top, dtype):
+    edges.check_top_repeats(rows, classes, top, dtype, DEV)

@@ -25,3 +25,7 @@ def test_masked_rest(host, dtype, masked, temperature):
 @pytest.mark.parametrize("dtype,masked", edges.MASKING)
 def test_masked_student(host, dtype, masked, temperature, rest):
     edges.check_masked_student(dtype, masked, temperature, rest, "cpu")
+
+
+def test_top_logits_repeat(host):
+    edges.check_top_repeats(3, 1541, 55, edges.F32, "cpu", turns=1)

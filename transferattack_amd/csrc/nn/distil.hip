@@ -652,18 +652,24 @@ __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {
         for (int i = 0; i < N; ++i) sum += exp2_hw((get(v, i) - ref) * c2);
         part += sum;
     };
+    // The copied elements come in the order the atomics gave out their places, another one in every run.  Their exponentials, at most 1,
+    // are rounded to multiples of 2^-40 (beside a sum of at least 1, the largest element's), so that the sum of all of them is
+    // exact in 64 bits and no order changes it.
+    double copied = 0.0;
+    static_assert(kHits * N <= 4096, "2^12 of them in multiples of 2^-40 are 52 bits");
     if (kept) {
 #pragma unroll
         for (int j = 0; j < KEPT; ++j) add(r.kept[j]);
         for (int e = tid; e < pairs; e += THREADS) {
             const float f = element_of(e);
-            if (key_of(f, hit_at[e / N] + e % N) < last) part += exp2_hw((f - ref) * c2);
+            if (key_of(f, hit_at[e / N] + e % N) < last) copied += (static_cast<double>(exp2_hw((f - ref) * c2)) + 4096.0) - 4096.0;
         }
+        copied = block_sum<WAVES>(copied, red_d);
     } else {
 #pragma unroll 1
         for (int j = 0; j < all; ++j) add(left(j));
     }
-    const double s = block_sum<WAVES>(static_cast<double>(part), red_d);
+    const double s = block_sum<WAVES>(static_cast<double>(part), red_d) + copied;
     if (tid == 0) {
         const double value = static_cast<double>(m) / static_cast<double>(a.temperature) + log(s);
         a.rest[row] = m == -INFINITY || m == INFINITY ? m : static_cast<float>(value);
