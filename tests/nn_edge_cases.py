@@ -2,11 +2,13 @@
 tier: the same functions, the device given by the caller.
 
 Bounds are counted as in nn_oracle: u = 2^-24 is half a step of fp32, t half a step of the tensors' type."""
+import pytest
 import torch
 
 import nn_oracle
 from nn_cases import BF16, F16, F32  # noqa: F401
 from transferattack_amd.distill import TopLogits, distillation_loss, distillation_loss_and_grad, top_logits
+from transferattack_amd.relative import RelativeBuckets, relative_attention, relative_attention_packed
 
 U = nn_oracle.U
 
@@ -87,3 +89,68 @@ def check_top_repeats(rows, classes, top, dtype, device, turns=12):
 
 
 REPEATED = [(2351, 1541, 55, F32), (325, 4721, 11, BF16), (900, 1000, 64, F32), (700, 30000, 40, F16)]
+
+
+def check_changed_before_backward(device):
+    """what a backward pass reads again is kept as autograd keeps its inputs: changed in between, it raises instead of mixing old and new"""
+    gen = torch.Generator().manual_seed(3)
+    q = torch.randn(2, 2, 70, 16, generator=gen).to(device).requires_grad_(True)
+    table = torch.randn(5, 2, generator=gen).to(device)
+    line = RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    lengths, start = torch.tensor([10, 20], dtype=torch.int32).to(device), torch.tensor([0, 3], dtype=torch.int32).to(device)
+    mask, added = torch.ones(70, 70, dtype=torch.bool).to(device), torch.zeros(2, 70, 70).to(device)
+    for name, changed in (("key_lengths", lengths), ("query_start", start), ("mask", mask), ("mask", added)):
+        out = relative_attention(q, q, q, table, line, **{name: changed})
+        changed.add_(1) if changed.dtype != torch.bool else changed.zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+    qkv = torch.randn(2, 70, 3, 2, 16, generator=gen).to(device).requires_grad_(True)
+    out = relative_attention_packed(qkv, table, line, mask=added, key_lengths=lengths)
+    lengths.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    x = torch.randn(3, 40, generator=gen).to(device).requires_grad_(True)
+    values, classes, rest, weight = (torch.randn(3, 4, generator=gen).to(device), torch.arange(12).view(3, 4).to(device), torch.zeros(3).to(device),
+                                     torch.ones(3).to(device))
+    for changed in (values, classes, rest, weight):
+        loss = distillation_loss(x, TopLogits(values, classes, rest, 2.0), weight=weight)
+        changed.mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def check_saved_tensor_hooks(device):
+    """what is kept passes by saved-tensor hooks (offloading, checkpoints), the options' tensors too"""
+    gen = torch.Generator().manual_seed(4)
+    q, table = torch.randn(2, 2, 9, 16, generator=gen).to(device).requires_grad_(True), torch.randn(5, 2, generator=gen).to(device)
+    plan = RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    lengths, mask = torch.tensor([9, 4], dtype=torch.int32).to(device), torch.zeros(9, 9).to(device)
+    x, answers = torch.randn(3, 40, generator=gen).to(device).requires_grad_(True), TopLogits(torch.zeros(3, 2).to(device), torch.tensor([[0, 1]] * 3).to(device))
+    weight = torch.ones(3).to(device)
+    steps = (lambda: torch.autograd.grad(relative_attention(q, q, q, table, plan, mask=mask, key_lengths=lengths).sum(), q)[0],
+             lambda: torch.autograd.grad(distillation_loss(x, answers, weight=weight), x)[0])
+    for step, kept in zip(steps, ((mask, lengths), (answers.values, answers.classes, weight))):
+        seen = []
+        plain = step()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.data_ptr()) or t.clone(), lambda t: t):
+            assert torch.equal(step(), plain)
+        assert {t.data_ptr() for t in kept} <= set(seen)
+
+
+def check_made_in_inference_mode(device):
+    """a teacher under torch.inference_mode, a mask and lengths made there: the student's step takes them, and has its own copy"""
+    gen = torch.Generator().manual_seed(5)
+    logits, q = torch.randn(3, 40, generator=gen).to(device), torch.randn(2, 2, 9, 16, generator=gen).to(device).requires_grad_(True)
+    table, plan = torch.randn(5, 2, generator=gen).to(device), RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    x = torch.randn(3, 40, generator=gen).to(device).requires_grad_(True)
+    with torch.inference_mode():
+        answers, weight = top_logits(logits, 5), torch.ones(3, device=device)
+        lengths, mask = torch.tensor([9, 4], dtype=torch.int32).to(device), torch.zeros(9, 9, device=device)
+    plain = TopLogits(answers.values.clone(), answers.classes.clone(), answers.rest.clone())
+    loss = distillation_loss(x, answers, weight=weight)
+    out = relative_attention(q, q, q, table, plan, mask=mask, key_lengths=lengths)
+    with torch.inference_mode():
+        answers.values.zero_(), weight.zero_(), lengths.zero_()
+    assert torch.equal(torch.autograd.grad(loss, x)[0], torch.autograd.grad(distillation_loss(x, plain, weight=torch.ones(3, device=device)), x)[0])
+    want = relative_attention(q, q, q, table, plan, mask=mask.clone(), key_lengths=torch.tensor([9, 4], dtype=torch.int32).to(device))
+    assert torch.equal(torch.autograd.grad(out.sum(), q)[0], torch.autograd.grad(want.sum(), q)[0])

@@ -23,3 +23,15 @@ def test_masked_student(dtype, masked, temperature, rest):
 @pytest.mark.parametrize("rows,classes,top,dtype", edges.REPEATED)
 def test_top_logits_repeat(rows, classes, top, dtype):
     edges.check_top_repeats(rows, classes, top, dtype, DEV)
+
+
+def test_changed_before_backward():
+    edges.check_changed_before_backward(DEV)
+
+
+def test_saved_tensor_hooks():
+    edges.check_saved_tensor_hooks(DEV)
+
+
+def test_made_in_inference_mode():
+    edges.check_made_in_inference_mode(DEV)

@@ -29,3 +29,15 @@ def test_masked_student(host, dtype, masked, temperature, rest):
 
 def test_top_logits_repeat(host):
     edges.check_top_repeats(3, 1541, 55, edges.F32, "cpu", turns=1)
+
+
+def test_changed_before_backward(host):
+    edges.check_changed_before_backward("cpu")
+
+
+def test_saved_tensor_hooks(host):
+    edges.check_saved_tensor_hooks("cpu")
+
+
+def test_made_in_inference_mode(host):
+    edges.check_made_in_inference_mode("cpu")

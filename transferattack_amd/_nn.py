@@ -118,5 +118,11 @@ def check_tensor(t, name, like=None, dtypes=None):
     return t
 
 
+def kept(*tensors):
+    """what ``ctx.save_for_backward`` takes: it refuses tensors made under ``torch.inference_mode`` (a teacher's answers), whose changes
+    nobody counts, so those are copied"""
+    return tuple(t.clone() if t is not None and t.is_inference() else t for t in tensors)
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()

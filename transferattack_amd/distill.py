@@ -152,16 +152,17 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, o):
         loss, stats, scale = _loss(rows, o, True)
-        ctx.save_for_backward(rows, stats, scale)
-        ctx.options = o
+        values, classes, rest, temperature, weight, reduction = o
+        ctx.save_for_backward(rows, stats, scale, *_nn.kept(values, classes, rest, weight))      # (one changed before the backward pass is an error)
+        ctx.options = temperature, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        rows, stats, scale = ctx.saved_tensors
-        o = ctx.options
-        weight, reduction = o[4], o[5]
+        rows, stats, scale, values, classes, rest, weight = ctx.saved_tensors
+        temperature, reduction = ctx.options
+        o = values, classes, rest, temperature, weight, reduction
         grad = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
         upstream = upstream.contiguous()
         factor = 1.0 / rows.shape[0] if reduction == "mean" and weight is None else 1.0

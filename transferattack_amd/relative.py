@@ -109,6 +109,21 @@ class _Call:
     """one call's options, checked"""
     __slots__ = ("buckets", "scale", "mask", "causal", "lengths", "start", "start_tensor")
 
+    def __init__(self):
+        self.mask = self.lengths = self.start_tensor = None
+
+    def split(self):
+        """(the options without their tensors, the tensors): a backward pass keeps the latter as autograd keeps inputs, so that one
+        changed in between is an error"""
+        o = _Call()
+        o.buckets, o.scale, o.causal, o.start = self.buckets, self.scale, self.causal, self.start
+        return o, (self.mask, self.lengths, self.start_tensor)
+
+    def joined(self, tensors):
+        o = self.split()[0]
+        o.mask, o.lengths, o.start_tensor = tensors
+        return o
+
 
 def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start):
     if not isinstance(buckets, RelativeBuckets):
@@ -127,7 +142,6 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
     o = _Call()
     o.buckets, o.causal = buckets, bool(causal)
     o.scale = dim ** -0.5 if scale is None else float(scale)
-    o.mask = None
     if mask is not None:
         _nn.check_tensor(mask, "mask", q, FLOATS + (torch.bool,))
         if mask.requires_grad:
@@ -139,13 +153,12 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
         if p == 0 or batch % p or h not in (1, heads) or i not in (1, m) or j not in (1, n):
             raise ValueError("mask %s does not fit batch %d, %d heads, %d queries, %d keys" % (tuple(mask.shape), batch, heads, m, n))
         o.mask = view
-    o.lengths = None
     if key_lengths is not None:
         _nn.check_tensor(key_lengths, "key_lengths", q, (torch.int32, torch.int64))
         if key_lengths.shape != (batch,):
             raise ValueError("key_lengths must be [%d], got %s" % (batch, tuple(key_lengths.shape)))
         o.lengths = key_lengths.to(torch.int32).contiguous()
-    o.start, o.start_tensor = 0, None
+    o.start = 0
     if isinstance(query_start, torch.Tensor):
         _nn.check_tensor(query_start, "query_start", q, (torch.int32, torch.int64))
         if query_start.shape != (batch,):
@@ -242,18 +255,18 @@ class _RelativeAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, o):
         out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
         stats = _forward(q, k, v, table, out, o, True)
-        ctx.save_for_backward(q, k, v, table, out, stats)
-        ctx.options = o
+        ctx.options, tensors = o.split()
+        ctx.save_for_backward(q, k, v, table, out, stats, *_nn.kept(*tensors))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, table, out, stats = ctx.saved_tensors
+        q, k, v, table, out, stats, *tensors = ctx.saved_tensors
         dq = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
         dk = _token_major(k.shape[0], k.shape[1], k.shape[2], k.shape[3], k)
         dv = _token_major(v.shape[0], v.shape[1], v.shape[2], v.shape[3], v)
-        dtable = _backward(q, k, v, table, out, stats, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options)
+        dtable = _backward(q, k, v, table, out, stats, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options.joined(tensors))
         return dq, dk, dv, dtable, None
 
 
@@ -268,19 +281,19 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, o):
         out, stats = _packed_forward(qkv, table, o, True)
-        ctx.save_for_backward(qkv, table, out, stats)
-        ctx.options = o
+        ctx.options, tensors = o.split()
+        ctx.save_for_backward(qkv, table, out, stats, *_nn.kept(*tensors))
         return out.flatten(2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        qkv, table, out, stats = ctx.saved_tensors
+        qkv, table, out, stats, *tensors = ctx.saved_tensors
         q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = dqkv.permute(2, 0, 3, 1, 4).unbind(0)
         grad = grad.reshape(out.shape).transpose(1, 2)
-        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options)
+        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options.joined(tensors))
         return dqkv, dtable, None
 
 
