@@ -154,3 +154,27 @@ def check_made_in_inference_mode(device):
     assert torch.equal(torch.autograd.grad(loss, x)[0], torch.autograd.grad(distillation_loss(x, plain, weight=torch.ones(3, device=device)), x)[0])
     want = relative_attention(q, q, q, table, plan, mask=mask.clone(), key_lengths=torch.tensor([9, 4], dtype=torch.int32).to(device))
     assert torch.equal(torch.autograd.grad(out.sum(), q)[0], torch.autograd.grad(want.sum(), q)[0])
+
+
+def check_forward_mode(device):
+    """tangents are refused where the tensor requires a gradient (by autograd) and where it does not"""
+    import torch.autograd.forward_ad as fwd
+    gen = torch.Generator().manual_seed(6)
+    q, x = torch.randn(2, 9, 3, 2, 16, generator=gen).to(device), torch.randn(3, 40, generator=gen).to(device)
+    table, plan = torch.randn(5, 2, generator=gen).to(device), RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    heads, weight = q[:, :, 0].transpose(1, 2).contiguous(), torch.ones(3).to(device)
+    answers = top_logits(x, 3)
+    attention = lambda q, k, v, t: relative_attention(q, k, v, t, plan)              # noqa: E731
+    for needs in (False, True):
+        with fwd.dual_level():
+            dual = lambda t: fwd.make_dual(t.clone().requires_grad_(needs), torch.ones_like(t))      # noqa: E731
+            for call in (lambda: attention(dual(heads), heads, heads, table), lambda: attention(heads, dual(heads), heads, table),
+                         lambda: attention(heads, heads, dual(heads), table), lambda: attention(heads, heads, heads, dual(table)),
+                         lambda: relative_attention_packed(dual(q), table, plan), lambda: relative_attention_packed(q, dual(table), plan),
+                         lambda: distillation_loss(dual(x), answers), lambda: distillation_loss_and_grad(dual(x), answers)):
+                with pytest.raises(RuntimeError):
+                    call()
+            attention(heads, heads, heads, table)        # no tangent among them: as ever
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError):
+            distillation_loss(x, answers, weight=fwd.make_dual(weight, weight))

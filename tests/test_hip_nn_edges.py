@@ -35,3 +35,7 @@ def test_saved_tensor_hooks():
 
 def test_made_in_inference_mode():
     edges.check_made_in_inference_mode(DEV)
+
+
+def test_forward_mode():
+    edges.check_forward_mode(DEV)

@@ -41,3 +41,7 @@ def test_saved_tensor_hooks(host):
 
 def test_made_in_inference_mode(host):
     edges.check_made_in_inference_mode("cpu")
+
+
+def test_forward_mode(host):
+    edges.check_forward_mode("cpu")

@@ -6,6 +6,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from ._hip import HipExtensionError
 
@@ -116,6 +117,14 @@ def check_tensor(t, name, like=None, dtypes=None):
     if dtypes is not None and t.dtype not in dtypes:
         raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(d).replace("torch.", "") for d in dtypes), t.dtype))
     return t
+
+
+def no_tangents(*tensors):
+    """forward-mode derivatives do not pass through the kernels: a dual tensor is refused rather than its tangent dropped"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives are not implemented for this operator")
 
 
 def kept(*tensors):

@@ -118,6 +118,7 @@ def _checked(rows, answers, weight, reduction):
         if weight.requires_grad:
             raise ValueError("the weights of the rows have no gradient")
         weight = weight.reshape(-1).contiguous()
+    _nn.no_tangents(rows, answers.values, answers.rest, weight)
     return (answers.values.contiguous(), answers.classes.contiguous(), None if answers.rest is None else answers.rest.contiguous(),
             answers.temperature, weight, reduction)
 
@@ -195,6 +196,7 @@ def distillation_loss_and_grad(logits, answers, weight=None, reduction="mean"):
     if reduction == "none":
         raise ValueError("reduction 'none' has no single loss to differentiate")
     rows = _rows_of(logits.detach() if isinstance(logits, torch.Tensor) else logits)
+    _nn.no_tangents(logits)                              # (detach drops them)
     o = _checked(rows, answers, weight, reduction)
     weight = o[4]
     n, dev = rows.shape[0], rows.device

@@ -331,6 +331,7 @@ def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=Fa
     if not 1 <= q.shape[3] <= MAX_DIM:
         raise ValueError("head dimension %d (1 .. %d)" % (q.shape[3], MAX_DIM))
     o = _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start)
+    _nn.no_tangents(q, k, v, table, mask)
     save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)
     if save and table.requires_grad and o.start_tensor is not None and buckets.distances:
         raise ValueError("the table's gradient needs one query_start for all sequences (an int)")
@@ -357,6 +358,7 @@ def relative_attention_packed(qkv, table, buckets, scale=None, mask=None, causal
         raise ValueError("qkv must be [batch, n, 3, heads, dim <= %d], got %s" % (MAX_DIM, tuple(qkv.shape)))
     q = qkv.detach().select(2, 0).transpose(1, 2)
     o = _options(q, q, table, buckets, scale, mask, causal, key_lengths, 0)
+    _nn.no_tangents(qkv, table, mask)
     save = torch.is_grad_enabled() and (qkv.requires_grad or table.requires_grad)
     dim, pad = qkv.shape[4], _padding(qkv)
     if pad:
