@@ -178,3 +178,26 @@ def check_forward_mode(device):
     with fwd.dual_level():
         with pytest.raises(NotImplementedError):
             distillation_loss(x, answers, weight=fwd.make_dual(weight, weight))
+
+
+def check_far_positions(device):
+    """positions near either end of 32 bits take the ends of the distances, in every kernel: few queries, tiles, windows, both ways"""
+    gen = torch.Generator().manual_seed(8)
+    table = torch.randn(5, 2, generator=gen).to(device)
+    low, high = -(1 << 31) + 1, (1 << 31) - 1
+    for m, n, first in ((3, 70, -2), (70, 80, -2), (70, 80, -(1 << 30) + 1)):
+        plan = RelativeBuckets.by_distance(torch.arange(5).to(device), first)
+        q, k = (torch.randn(2, 2, t, 16, generator=gen).to(device).requires_grad_(True) for t in (m, n))
+        for start, bucket in ((low, 4), (high, 0)):
+            every = RelativeBuckets.from_index(torch.full((m, n), bucket).to(device))
+            out = relative_attention(q, k, k, table, plan, query_start=torch.tensor([start, start], dtype=torch.int32).to(device))
+            want = relative_attention(q, k, k, table, every)
+            # the same scores plus the same constant: what differs is which kernel adds them up, some 100 roundings
+            assert (out - want).abs().max() <= 200 * U * want.abs().max()
+            for a, b in zip(torch.autograd.grad(out.square().sum(), (q, k)), torch.autograd.grad(want.square().sum(), (q, k))):
+                assert (a - b).abs().max() <= 1000 * U * b.abs().max()
+    plan = RelativeBuckets.by_distance(torch.arange(5).to(device), -(1 << 30) + 1)
+    q = torch.randn(2, 2, 9, 16, generator=gen).to(device)
+    got = relative_attention(q, q, q, table, plan, query_start=-(1 << 30) + 1)
+    want = relative_attention(q, q, q, table, RelativeBuckets.from_index(torch.full((9, 9), 4).to(device)))
+    assert torch.equal(got, want)

@@ -39,3 +39,7 @@ def test_made_in_inference_mode():
 
 def test_forward_mode():
     edges.check_forward_mode(DEV)
+
+
+def test_far_positions():
+    edges.check_far_positions(DEV)

@@ -45,3 +45,7 @@ def test_made_in_inference_mode(host):
 
 def test_forward_mode(host):
     edges.check_forward_mode("cpu")
+
+
+def test_far_positions(host):
+    edges.check_far_positions("cpu")

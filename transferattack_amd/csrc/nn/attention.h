@@ -207,9 +207,13 @@ __device__ __forceinline__ void stage_bias(const AttentionArgs& a, float* lds, i
     }
 }
 
-// positions may lie anywhere: clamped to where adding a token's number (below 2^30) can neither overflow nor change the answer
-__device__ __forceinline__ int clamp_entry(int64_t e) {
-    return static_cast<int>(max(-(static_cast<int64_t>(1) << 30), min(e, static_cast<int64_t>(0x7FFFFFFF))));
+// Positions may lie anywhere: clamped to where adding (a query's column, rows count up) or subtracting (a key's, they count down) a
+// token's number, below 2^30 and a tile, can neither overflow nor change the answer; there are fewer than 2^29 distances.
+__device__ __forceinline__ int clamp_query_entry(int64_t e) {
+    return static_cast<int>(max(-(static_cast<int64_t>(1) << 30) - 64, min(e, static_cast<int64_t>(1) << 29)));
+}
+__device__ __forceinline__ int clamp_key_entry(int64_t e) {
+    return static_cast<int>(max(-(static_cast<int64_t>(1) << 29), min(e, static_cast<int64_t>(0x7FFFFFFF))));
 }
 __device__ __forceinline__ int clamp_token(int64_t t) {
     return static_cast<int>(max(static_cast<int64_t>(-1), min(t, static_cast<int64_t>(1) << 30)));
@@ -236,13 +240,13 @@ struct Column {
 __device__ __forceinline__ Column query_column(const AttentionArgs& a, const float* bias, int64_t b, int head, int query, int start,
                                                int keys) {
     const int64_t position = static_cast<int64_t>(start) + query;
-    return Column{bias, head, clamp_entry(-position - a.first), a.causal ? min(clamp_token(position), keys - 1) : keys - 1,
+    return Column{bias, head, clamp_query_entry(-position - a.first), a.causal ? min(clamp_token(position), keys - 1) : keys - 1,
                   a.distances ? nullptr : static_cast<const unsigned short*>(a.index) + query * a.index_stride,
                   a.mask_kind ? b % a.mask_period * a.mask_sb + head * a.mask_sh + query * a.mask_sm : 0};
 }
 __device__ __forceinline__ Column key_column(const AttentionArgs& a, const float* bias, int64_t b, int head, int key, int start) {
     const int64_t lead = static_cast<int64_t>(key) - start;
-    return Column{bias, head, clamp_entry(lead - a.first), a.causal ? clamp_token(lead) : 0,
+    return Column{bias, head, clamp_key_entry(lead - a.first), a.causal ? clamp_token(lead) : 0,
                   a.distances ? nullptr : static_cast<const unsigned short*>(a.index_t) + key * a.index_t_stride,
                   a.mask_kind ? b % a.mask_period * a.mask_sb + head * a.mask_sh + key * a.mask_sn : 0};
 }
