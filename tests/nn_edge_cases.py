@@ -201,3 +201,17 @@ def check_far_positions(device):
     got = relative_attention(q, q, q, table, plan, query_start=-(1 << 30) + 1)
     want = relative_attention(q, q, q, table, RelativeBuckets.from_index(torch.full((9, 9), 4).to(device)))
     assert torch.equal(got, want)
+
+
+def check_64_bit_positions(device):
+    """lengths and positions of 64 bits beyond what 32 hold: all keys, none, the ends of the distances"""
+    gen = torch.Generator().manual_seed(7)
+    q, k = torch.randn(4, 2, 3, 16, generator=gen).to(device), torch.randn(4, 2, 7, 16, generator=gen).to(device)
+    table, plan = torch.randn(5, 2, generator=gen).to(device), RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    ints = lambda *v: torch.tensor(v).to(device)         # noqa: E731
+    top = torch.iinfo(torch.int64).max
+    got = relative_attention(q, k, k, table, plan, key_lengths=ints(top, 1 << 32, -(1 << 32) + 3, -top - 1))
+    assert torch.equal(got, relative_attention(q, k, k, table, plan, key_lengths=ints(7, 7, 0, 0).int()))
+    for causal in (False, True):
+        got = relative_attention(q, k, k, table, plan, causal=causal, query_start=ints(top, 1 << 32, -(1 << 32) + 3, -top - 1))
+        assert torch.equal(got, relative_attention(q, k, k, table, plan, causal=causal, query_start=ints(100, 100, -100, -100)))

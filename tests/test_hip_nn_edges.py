@@ -43,3 +43,7 @@ def test_forward_mode():
 
 def test_far_positions():
     edges.check_far_positions(DEV)
+
+
+def test_64_bit_positions():
+    edges.check_64_bit_positions(DEV)

@@ -49,3 +49,7 @@ def test_forward_mode(host):
 
 def test_far_positions(host):
     edges.check_far_positions("cpu")
+
+
+def test_64_bit_positions(host):
+    edges.check_64_bit_positions("cpu")

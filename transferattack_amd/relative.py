@@ -125,6 +125,11 @@ class _Call:
         return o
 
 
+def _int32(t, low, high):
+    """as the kernels take it; 64-bit numbers past ``low`` or ``high`` mean the same as those"""
+    return (t if t.dtype == torch.int32 else t.clamp(low, high).to(torch.int32)).contiguous()
+
+
 def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start):
     if not isinstance(buckets, RelativeBuckets):
         raise TypeError("buckets must be RelativeBuckets, got %s" % type(buckets).__name__)
@@ -157,13 +162,13 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
         _nn.check_tensor(key_lengths, "key_lengths", q, (torch.int32, torch.int64))
         if key_lengths.shape != (batch,):
             raise ValueError("key_lengths must be [%d], got %s" % (batch, tuple(key_lengths.shape)))
-        o.lengths = key_lengths.to(torch.int32).contiguous()
+        o.lengths = _int32(key_lengths, 0, n)
     o.start = 0
     if isinstance(query_start, torch.Tensor):
         _nn.check_tensor(query_start, "query_start", q, (torch.int32, torch.int64))
         if query_start.shape != (batch,):
             raise ValueError("query_start must be an int or [%d], got %s" % (batch, tuple(query_start.shape)))
-        o.start_tensor = query_start.to(torch.int32).contiguous()
+        o.start_tensor = _int32(query_start, -(1 << 31) + 1, (1 << 31) - 1)
     else:
         o.start = int(query_start)
         if abs(o.start) >= 1 << 30:
