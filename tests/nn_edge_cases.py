@@ -215,3 +215,18 @@ def check_64_bit_positions(device):
     for causal in (False, True):
         got = relative_attention(q, k, k, table, plan, causal=causal, query_start=ints(top, 1 << 32, -(1 << 32) + 3, -top - 1))
         assert torch.equal(got, relative_attention(q, k, k, table, plan, causal=causal, query_start=ints(100, 100, -100, -100)))
+
+
+def check_rows_of_answers(device):
+    """a batch of answers indexed and iterated like a batch of labels"""
+    answers = TopLogits(torch.arange(6.0).view(3, 2).to(device), torch.arange(6).view(3, 2).to(device), torch.arange(3.0).to(device), 2.0)
+    parts = list(answers)
+    assert len(parts) == 3 and all(len(p) == 1 and torch.equal(p.values, answers.values[i:i + 1]) and torch.equal(p.rest, answers.rest[i:i + 1])
+                                   for i, p in enumerate(parts))
+    assert torch.equal(answers[-1].values, answers[2].values) and torch.equal(answers[-3].values, answers[0].values)
+    for at in (3, -4, 1 << 40):
+        with pytest.raises(IndexError):
+            answers[at]
+    assert list(answers[:0]) == [] and len(answers[torch.tensor([True, False, True]).to(device)]) == 2 and len(answers[torch.tensor([2, 2]).to(device)]) == 2
+    one, two, three = answers
+    assert torch.equal(three.classes, answers[2:].classes)

@@ -47,3 +47,7 @@ def test_far_positions():
 
 def test_64_bit_positions():
     edges.check_64_bit_positions(DEV)
+
+
+def test_rows_of_answers():
+    edges.check_rows_of_answers(DEV)

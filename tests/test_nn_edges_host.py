@@ -53,3 +53,7 @@ def test_far_positions(host):
 
 def test_64_bit_positions(host):
     edges.check_64_bit_positions("cpu")
+
+
+def test_rows_of_answers(host):
+    edges.check_rows_of_answers("cpu")

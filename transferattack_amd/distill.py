@@ -8,6 +8,8 @@ takes labels (transferattack/attack.py:155-162): untargeted, it moves the surrog
 ([labels, answers]), towards it.
 
 No fallback: tensors must be on a HIP device."""
+import operator
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -52,8 +54,11 @@ class TopLogits:
         return self.values.shape[0]
 
     def __getitem__(self, rows):
-        if isinstance(rows, int):
-            rows = slice(rows, rows + 1 or None)
+        if hasattr(rows, "__index__") and not isinstance(rows, (bool, torch.Tensor)):      # one row, still as a batch
+            at, n = operator.index(rows), len(self)
+            if not -n <= at < n:                         # (what ends an iteration)
+                raise IndexError("row %d of %d" % (at, n))
+            rows = slice(at % n, at % n + 1)
         return self._each(lambda t: t[rows])
 
     def repeat(self, times):
