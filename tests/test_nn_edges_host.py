@@ -1,5 +1,6 @@
 """nn_edge_cases where there is no GPU: the kernel sources compiled for the host, driven through the package's binding."""
 import os
+import subprocess
 import sys
 
 import pytest
@@ -57,3 +58,14 @@ def test_64_bit_positions(host):
 
 def test_rows_of_answers(host):
     edges.check_rows_of_answers("cpu")
+
+
+def test_import_without_a_gpu_build_of_torch():
+    """the package, its surrogates among it, imports where torch has no functions of a GPU"""
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice', '_cuda_setDevice'):\n"
+            "    hasattr(torch._C, n) and delattr(torch._C, n)\n"
+            "import transferattack_amd.backbones, transferattack_amd.relative, transferattack_amd.distill, transferattack_amd.attack\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stderr[-2000:]

@@ -92,17 +92,16 @@ def _on_device(t, name):
         raise HipExtensionError("%s is on %s: the HIP path needs tensors on a HIP device (no CPU fallback)" % (name, t.device))
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream       # what torch.cuda.current_stream(dev).cuda_stream is, without the objects
-
-
 def _launch(name, like, *args):
     fn = getattr(_lib or load(), name)
     dev = like.get_device()
+    # (what torch.cuda.current_stream(dev).cuda_stream is, without the objects; torch builds without a GPU do not have it)
+    raw_stream = torch._C._cuda_getCurrentRawStream
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):                   # the launch needs the tensor's device current in this thread
-            rc = fn(*args, _raw_stream(dev))
+            rc = fn(*args, raw_stream(dev))
     else:
-        rc = fn(*args, _raw_stream(dev))
+        rc = fn(*args, raw_stream(dev))
     if rc != 0:
         _check(rc, name)
 
