@@ -230,3 +230,51 @@ def check_rows_of_answers(device):
     assert list(answers[:0]) == [] and len(answers[torch.tensor([True, False, True]).to(device)]) == 2 and len(answers[torch.tensor([2, 2]).to(device)]) == 2
     one, two, three = answers
     assert torch.equal(three.classes, answers[2:].classes)
+
+
+# The attacks that take a victim's answers, checked against themselves: with one class answered and no mass for the others the
+# loss at temperature 1 is -log q of that class, cross entropy on its label.
+REFUSING = {"mig", "vaifgsm", "anda", "foolmix", "su", "everywhere", "adaea", "smer"}
+ENSEMBLES = {"ens", "svre", "cwa", "adaea", "smer"}
+SMALL = dict(epoch=1, num_neighbor=2, num_sample=3, num_scale=2, num_warping=2, num_spectrum=2, num_ens=2, transpoint=0, adv_steps=2, max_iter=2,
+             num_sample_neighbor=2, num_sample_operator=2, K=2)
+
+
+def attack_on_toys(name, device, **kw):
+    import inspect
+    import transferattack_amd as ta
+    from transferattack_amd import backbones
+    from transferattack_amd.utils import EnsembleModel, wrap_model
+    base = ta.load_attack_class(name)
+    models = [backbones.create("toy_cnn", seed=3 + i, verbose=False) for i in range(2 if name in ENSEMBLES else 1)]
+
+    def load_model(self, model_name):
+        wrapped = [wrap_model(m.eval().to(device)) for m in models]
+        return EnsembleModel(wrapped) if name in ENSEMBLES else wrapped[0]
+
+    kw = dict({k: v for k, v in SMALL.items() if k in inspect.signature(base.__init__).parameters}, **kw)
+    cls = type("Toy" + base.__name__, (base,), {"load_model": load_model})
+    return cls(model_name=["a", "b"] if name in ENSEMBLES else "injected", **kw)
+
+
+def check_attack_on_answers(name, device):
+    import random
+    import numpy as np
+    if name in REFUSING:
+        with pytest.raises(Exception, match="Unsupported loss distillation|unexpected keyword argument 'loss'"):
+            attack_on_toys(name, device, loss="distillation", **({"targeted": True} if name == "everywhere" else {}))
+        return
+    x = torch.randint(0, 256, (2, 3, 224, 224), generator=torch.Generator().manual_seed(0)).float() / 255
+    label = torch.tensor([3, 7])
+    answers = TopLogits(torch.zeros(2, 1), label[:, None])
+    got = {}
+    for loss, y in (("crossentropy", label), ("distillation", answers)):
+        atk = attack_on_toys(name, device, loss=loss)
+        torch.manual_seed(5), np.random.seed(5), random.seed(5)
+        got[loss] = atk(x, y).cpu()
+    a, b = got["crossentropy"], got["distillation"]
+    assert float(b.abs().max()) > 0 and float(b.abs().max()) <= 16 / 255 + 1e-7
+    # the two gradients are the same but for a few roundings of 2^-24: steps of the gradient's sign differ where it is within those of 0,
+    # steps of its value by as much
+    differ = float(((a - b).abs() > 1e-5).float().mean())
+    assert differ <= 0.02, differ

@@ -2,6 +2,7 @@
 import pytest
 
 import nn_edge_cases as edges
+import transferattack_amd
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -51,3 +52,8 @@ def test_64_bit_positions():
 
 def test_rows_of_answers():
     edges.check_rows_of_answers(DEV)
+
+
+@pytest.mark.parametrize("name", sorted(transferattack_amd.attack_zoo))
+def test_attack_on_answers(name):
+    edges.check_attack_on_answers(name, DEV)

@@ -6,8 +6,10 @@ import sys
 import pytest
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "hipcpu_nn"))
+import host_kernels                  # noqa: E402
 import nn_edge_cases as edges        # noqa: E402
 import nn_host_build                 # noqa: E402
+import transferattack_amd            # noqa: E402
 
 
 @pytest.fixture
@@ -69,3 +71,9 @@ def test_import_without_a_gpu_build_of_torch():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=600)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("name", sorted(transferattack_amd.attack_zoo))
+def test_attack_on_answers(host, name, monkeypatch):
+    host_kernels.install(monkeypatch)
+    edges.check_attack_on_answers(name, "cpu")

@@ -94,6 +94,10 @@ _flags_before_deterministic = None          # the process-wide torch flags deter
 class Attack(object):
     """Base class for all attacks (same constructor as transferattack/attack.py:12-38)."""
 
+    #: whether answers (distill.TopLogits, ``loss='distillation'``) may stand in the labels' place: False where an attack
+    #: computes a loss of its own or reads class numbers from the labels
+    takes_answers = True
+
     def __init__(self, attack, model_name, epsilon, targeted, random_start, norm, loss, device=None):
         if norm not in ['l2', 'linfty']:
             raise Exception("Unsupported norm {}".format(norm))
@@ -370,6 +374,8 @@ class Attack(object):
         if loss == 'crossentropy':
             return nn.CrossEntropyLoss()
         if loss == 'distillation':                      # labels are a victim's answers (distill.TopLogits)
+            if not self.takes_answers:
+                raise Exception("Unsupported loss {}: {} has a loss of its own or reads class numbers".format(loss, type(self).__name__))
             from .distill import DistillationLoss
             return DistillationLoss()
         raise Exception("Unsupported loss {}".format(loss))

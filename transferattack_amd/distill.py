@@ -3,9 +3,10 @@
 A black-box victim answers an image with its best classes and their scores.  ``TopLogits`` holds such answers (``top_logits``
 makes them from a local model's logits), ``distillation_loss`` is T^2 KL(teacher || student) on them -- the teacher's distribution
 on the classes answered, and, where the mass it leaves to all others is known, on one more bin for those -- with its gradient in
-the student's logits.  Every attack takes ``loss='distillation'`` and then answers in the place of labels (``DistillationLoss``), as 'crossentropy'
-takes labels (transferattack/attack.py:155-162): untargeted, it moves the surrogate away from what the victim answered; targeted
-([labels, answers]), towards it.
+the student's logits (the answers have none).  Attacks that take a loss take ``loss='distillation'`` and then answers in the place of labels
+(``DistillationLoss``), as 'crossentropy' takes labels (transferattack/attack.py:155-162): untargeted, they move the surrogate away from
+what the victim answered; targeted ([labels, answers]), towards it.  Those with a loss of their own, or that read class numbers, refuse it
+when constructed (``Attack.takes_answers``).
 
 No fallback: tensors must be on a HIP device."""
 import operator

@@ -12,6 +12,8 @@ from ..attack import Attack
 class AdaEA(Attack):
     """Official arguments: epsilon=16/255, alpha=1.6/255, epoch=10, decay=1.0, beta=10, threshold=-0.3."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=1.6/255, epoch=10, decay=1.0, targeted=False,
                  random_start=True, beta=10, threshold=-0.3, norm='linfty', loss='crossentropy', device=None,
                  attack='AdaEA', **kwargs):

@@ -30,6 +30,8 @@ class Weight_Selection(nn.Module):
 class SMER(Attack):
     """Official arguments: epsilon=16/255, alpha=1.6/255, epoch=10, decay=1.0, random_start=True."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=1.6/255, epoch=10, decay=1.0, targeted=False,
                  random_start=True, norm='linfty', loss='crossentropy', device=None, attack='SMER', **kwargs):
         super().__init__(attack, model_name, epsilon, targeted, random_start, norm, loss, device)

@@ -16,6 +16,8 @@ from ..attack import Attack
 class ANDA(Attack):
     """Official arguments: epsilon=16/255, alpha=1.6/255, epoch=10, n_ens=25, aug_max=0.3, sample=False."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=1.6/255, epoch=10, n_ens=25, aug_max=0.3, sample=False,
                  targeted=False, random_start=False, norm='linfty', loss='crossentropy', device=None, attack='ANDA', **kwargs):
         super().__init__(attack, model_name, epsilon, targeted, random_start, norm, loss, device)

@@ -22,6 +22,8 @@ class Foolmix(Attack):
     """Official arguments: epsilon=16/255, alpha=1.6/255, epoch=10, decay=1., m=5, n=3, z=1, k=5, zeta=0.2, beta=1.0,
     gamma=0.1."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=1.6/255, epoch=10, decay=1., targeted=False, random_start=False,
                  norm='linfty', loss='crossentropy', device=None, attack='Foolmix', m=5, n=3, z=1, k=5, zeta=0.2, beta=1.0,
                  gamma=0.1, print_timing=True, use_amp=True, use_cache=False, grad_chunk_size=16, **kwargs):

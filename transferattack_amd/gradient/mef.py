@@ -21,11 +21,9 @@ class MEF(Attack):
         self.inner_decay, self.num_neighbor = inner_decay, num_neighbor
 
     def loss_function(self, loss):
-        if loss == 'crossentropy':
-            return nn.CrossEntropyLoss()
         if loss == 'crossentropy_no_reduction':
             return nn.CrossEntropyLoss(reduction='none')
-        raise Exception("Unsupported loss {}".format(loss))
+        return super().loss_function(loss)                   # (the mean taken below leaves a mean as it is)
 
     def get_conditional_sampled_points(self, delta, grad_pgia):
         """the ``num_neighbor`` sampling points: uniform in the gamma-ball around delta, then pushed by kesai along the

@@ -11,6 +11,8 @@ from .mifgsm import MIFGSM
 class MIG(MIFGSM):
     """Official arguments: epsilon=16/255, alpha=epsilon/epoch, epoch=10, decay=1., s_factor=20."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=1.6/255, epoch=10, decay=1., s_factor=20, targeted=False,
                  random_start=False, norm='linfty', loss='crossentropy', device=None, attack='MIG', **kwargs):
         super().__init__(model_name, epsilon, epsilon / epoch, epoch, decay, targeted, random_start, norm, loss, device,

@@ -12,6 +12,8 @@ from .. import _hip
 class VAIFGSM(Attack):
     """Official arguments: epsilon=16/255, alpha=0.007, epoch=20, aux_num=3."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=0.007, epoch=20, aux_num=3, targeted=False, random_start=False,
                  norm='linfty', loss='crossentropy', device=None, attack='VA-I-FGSM', **kwargs):
         super().__init__(attack, model_name, epsilon, targeted, random_start, norm, loss, device)

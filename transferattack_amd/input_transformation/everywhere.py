@@ -37,6 +37,8 @@ config = {
 class EverywhereAttack(Attack):
     """Official arguments: epsilon=16/255, lr=1.6/255, epoch=300, num_blocks=16, N=9, img_size=224 (targeted)."""
 
+    takes_answers = False
+
     def __init__(self, model_name, targeted, attack="everywhere", img_size=224, epsilon=16/255, lr=1.6/255, epoch=300,
                  num_blocks=16, N=9):
         super().__init__(attack, model_name, epsilon, targeted, random_start=True, norm='linfty', loss='crossentropy',

@@ -68,6 +68,8 @@ class SU(MIFGSM):
     """Official arguments: epsilon=16/255, alpha=2/255, epoch=300, decay=1, coef=0.001, scale=(0.1, 0.0), depth=3
     (layer3 of ResNet-50), targeted."""
 
+    takes_answers = False
+
     def __init__(self, model_name, epsilon=16/255, alpha=2/255, epoch=300, decay=1., coef=0.001, scale=(0.1, 0.0), depth=3,
                  targeted=True, random_start=False, norm='linfty', loss='crossentropy', device=None, attack='SU', **kwargs):
         super().__init__(model_name, epsilon, alpha, epoch, decay, targeted, random_start, norm, loss, device, attack)
