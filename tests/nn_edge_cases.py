@@ -23,7 +23,7 @@ def distil_rows_64(x, values, classes, rest, temperature):
     answered = torch.zeros_like(x, dtype=torch.bool).scatter_(1, classes.cpu(), True)
     log_rest = log_q.masked_fill(answered, -torch.inf).logsumexp(1, keepdim=True)
     at = log_q.gather(1, classes.cpu())
-    w = torch.softmax(x.masked_fill(answered, -torch.inf), 1)      # (log_q - log_rest would lose log n beside a masking constant)
+    w = torch.softmax(x.masked_fill(answered, -torch.inf), 1).nan_to_num(0.0)      # (0: no other class; log_q - log_rest would lose log n beside a masking constant)
     p = log_p.exp()
     p_rest = torch.zeros_like(log_rest)
     if rest is not None:
@@ -278,3 +278,33 @@ def check_attack_on_answers(name, device):
     # steps of its value by as much
     differ = float(((a - b).abs() > 1e-5).float().mean())
     assert differ <= 0.02, differ
+
+
+def check_near_the_teacher(rest, twice, device):
+    """a student within 1e-6 of its teacher: the gradients of the classes answered, q - p, are a millionth of either, and both forms have
+    them to what the row's sums leave.  With every class answered all of it is 64-bit, and only the result is rounded.  With more
+    classes the sum of the others is off by r = 200 u + (2 |x - m| / T + 4) u at most, so q by r q_R q, weighted like the terms"""
+    gen = torch.Generator().manual_seed(10)
+    rows, n = 4, 50
+    top = 10 if rest else n
+    teacher = torch.randn(rows, n, generator=gen, dtype=torch.float64)
+    student = (teacher + 1e-6 * torch.randn(rows, n, generator=gen, dtype=torch.float64)).float()
+    values, classes = torch.topk(teacher.float(), top, dim=1)
+    left = teacher.float().double().scatter(1, classes, -torch.inf).logsumexp(1).float() if rest else None
+    if twice:                                            # a class given twice, each time with half of its mass
+        values[:, 1], classes[:, 1] = values[:, 0], classes[:, 0]
+        values[:, :2] -= torch.tensor(2.0).log()
+    loss, grad, w, log_rest, p_rest = distil_rows_64(student, values, classes, left, 1.0)
+    q = torch.log_softmax(student.double(), 1).exp()
+    away = (student.double().amax(1, keepdim=True) - student.double())
+    r = 200 * U + ((2 * away + 4) * U * w).sum(1, keepdim=True) if rest or twice else torch.zeros(rows, 1, dtype=torch.float64)
+    off = (r * log_rest.exp() * q + (r + (2 * away + 6) * U) * w * (log_rest.exp() + p_rest) * (w > 0) + 3 * U * grad.abs() + 1e-13)
+    answers = TopLogits(values.to(device), classes.to(device), None if left is None else left.to(device), 1.0)
+    x = student.to(device).requires_grad_(True)
+    (dx,) = torch.autograd.grad(distillation_loss(x, answers, reduction="sum"), x)
+    both = distillation_loss_and_grad(x, answers, reduction="sum")[1]
+    for g in (dx, both):
+        assert ((g.cpu().double() - grad).abs() <= off).all(), ((g.cpu().double() - grad).abs() / off).max()
+    # the two forms have the same numbers of the classes answered, but for what 1 / Z kept in two parts leaves (2^-48) and one rounding
+    at = classes.to(device)
+    assert ((dx - both).gather(1, at).abs() <= 2 * U * both.gather(1, at).abs() + 1e-13).all()

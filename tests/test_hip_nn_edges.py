@@ -57,3 +57,8 @@ def test_rows_of_answers():
 @pytest.mark.parametrize("name", sorted(transferattack_amd.attack_zoo))
 def test_attack_on_answers(name):
     edges.check_attack_on_answers(name, DEV)
+
+
+@pytest.mark.parametrize("rest,twice", [(False, False), (True, False), (False, True), (True, True)])
+def test_near_the_teacher(rest, twice):
+    edges.check_near_the_teacher(rest, twice, DEV)

@@ -77,3 +77,8 @@ def test_import_without_a_gpu_build_of_torch():
 def test_attack_on_answers(host, name, monkeypatch):
     host_kernels.install(monkeypatch)
     edges.check_attack_on_answers(name, "cpu")
+
+
+@pytest.mark.parametrize("rest,twice", [(False, False), (True, False), (False, True), (True, True)])
+def test_near_the_teacher(host, rest, twice):
+    edges.check_near_the_teacher(rest, twice, "cpu")

@@ -39,7 +39,9 @@ struct DistilArgs {
     int64_t grad_stride;
 };
 
-constexpr int kStats = 5;                                // m, (q_R - p_R) / s, M = max over all, 1 / Z, whether a class repeats
+// m, (q_R - p_R) / s, M = max over all, 1 / Z in two parts (q - p of a class answered nearly cancels near the teacher), the first one
+// negative where a class repeats
+constexpr int kStats = 5;
 
 __device__ __forceinline__ int class_at(const DistilArgs& a, int64_t row, int i) {
     const int64_t at = row * a.k + i;
@@ -323,8 +325,9 @@ __global__ __launch_bounds__(THREADS, 4) void distil_rows(DistilArgs a) {
                 stats[0] = ref;
                 stats[1] = static_cast<float>(kappa);
                 stats[2] = static_cast<float>(m_all);
-                stats[3] = static_cast<float>(inv_z);
-                stats[4] = repeats ? 1.0f : 0.0f;
+                const float high = static_cast<float>(inv_z);
+                stats[3] = repeats ? -high : high;
+                stats[4] = static_cast<float>(inv_z - static_cast<double>(high));
             }
             other_factor = static_cast<float>(kappa * coef);
         }
@@ -369,8 +372,9 @@ __global__ __launch_bounds__(THREADS) void distil_backward(DistilArgs a) {
         return;
     }
     const float* stats = a.stats + row * kStats;
-    const float ref = stats[0], kappa = stats[1], m_all = stats[2], inv_z = stats[3];
-    const bool repeats = stats[4] != 0.0f;
+    const float ref = stats[0], kappa = stats[1], m_all = stats[2];
+    const bool repeats = stats[3] < 0.0f;
+    const double inv_z = static_cast<double>(fabsf(stats[3])) + static_cast<double>(stats[4]);
     double coef = a.temperature * static_cast<double>(w) * static_cast<double>(a.factor);
     if (a.scale) coef *= static_cast<double>(*a.scale);
     if (a.upstream) coef *= static_cast<double>(a.upstream[a.upstream_per_row ? row : 0]);
