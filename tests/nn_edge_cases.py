@@ -308,3 +308,54 @@ def check_near_the_teacher(rest, twice, device):
     # the two forms have the same numbers of the classes answered, but for what 1 / Z kept in two parts leaves (2^-48) and one rounding
     at = classes.to(device)
     assert ((dx - both).gather(1, at).abs() <= 2 * U * both.gather(1, at).abs() + 1e-13).all()
+
+
+def attention_64(q, k, v, grad, bias):
+    """softmax(q k^T dim^-0.5 + bias) v and its gradients in 64 bits (every pair seen), with what the kernels' 32-bit arithmetic may leave at the
+    steps of nn_oracle's docstring: scores, probabilities (rel), dp, delta and ds.  -> dict"""
+    q, k, v, grad, bias = (x.detach().cpu().double() for x in (q, k, v, grad, bias))
+    dim, n, m, scale = q.shape[-1], k.shape[-2], q.shape[-2], q.shape[-1] ** -0.5
+    s = q @ k.transpose(-2, -1) * scale + bias
+    size = q.abs() @ k.abs().transpose(-2, -1) * scale + bias.abs()
+    p = s.softmax(-1)
+    rel = 2 * (dim + 4) * U * size.amax(-1, keepdim=True) + 4 * U * (s.amax(-1, keepdim=True) - s).clamp(0, 200) + (n + 8) * U
+    out, dp = p @ v, grad @ v.transpose(-2, -1)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    dp_err = (dim + 4) * U * (grad.abs() @ v.abs().transpose(-2, -1))
+    delta_err = (p * (rel + n * U) * dp.abs() + p * dp_err).sum(-1, keepdim=True)
+    ds_err = p * rel * (dp - delta).abs() + p * (1 + rel) * (dp_err + delta_err) + 2 * U * p * (dp.abs() + delta.abs()) + 2.0 ** -120
+    return dict(q=q, k=k, v=v, grad=grad, p=p, rel=rel, out=out, ds=ds, ds_err=ds_err, scale=scale, n=n, m=m, dim=dim,
+                dq=ds @ k * scale, dk=ds.transpose(-2, -1) @ q * scale, dv=p.transpose(-2, -1) @ grad)
+
+
+def dq_bound(x, t, smallest=0.0):
+    """of dq where ds is rounded once (t of it) and delta is sum p dp: the delta that ds is formed with is out . grad, off by what out is
+    rounded by twice (its probabilities, itself); put right it leaves that times t, of ds and of p.  `smallest`: half a step of the
+    type's smallest numbers, for the result"""
+    out_err = (x["p"] * (x["rel"] + t + x["n"] * U)) @ x["v"].abs() + t * x["out"].abs()
+    apart = (out_err * x["grad"].abs()).sum(-1, keepdim=True) + (x["dim"] + 4) * U * (x["out"] * x["grad"]).abs().sum(-1, keepdim=True)
+    terms = x["ds_err"] + (t + x["n"] * U) * x["ds"].abs() + (2 * t + x["n"] * U) * x["p"] * apart
+    return terms @ x["k"].abs() * x["scale"] + (t + 2 * U) * x["dq"].abs() + smallest
+
+
+def check_dq_of_few_heavy_keys(dtype, pairs, spread, device):
+    """200 keys of which a few hold a row's mass (queries `spread` times as large): dp - delta of those nearly cancels, so delta must not
+    come from the rounded output"""
+    gen = torch.Generator().manual_seed(12)
+    m, n, dim = 70, 200, 64
+    q, k, v, grad = (torch.randn(1, 2, t, dim, generator=gen) for t in (m, n, n, m))
+    q, k, v, grad = (t.to(dtype) for t in (q * spread, k, v, grad))
+    table = torch.randn(5, 2, generator=gen)
+    if pairs:
+        index = torch.randint(0, 5, (m, n), generator=gen)
+        plan = RelativeBuckets.from_index(index.to(device))
+    else:
+        index = (torch.arange(n)[None] - torch.arange(m)[:, None] + 2).clamp(0, 4)
+        plan = RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    leaf = q.to(device).requires_grad_(True)
+    out = relative_attention(leaf, k.to(device), v.to(device), table.to(device), plan)
+    (dq,) = torch.autograd.grad(out, leaf, grad.to(device))
+    x = attention_64(q, k, v, grad, table[index].movedim(-1, 0))
+    off, bound = (dq.cpu().double() - x["dq"]).abs(), dq_bound(x, nn_oracle.half_step(dtype), 2.0 ** -25 if dtype == F16 else 0.0)
+    assert (off <= bound).all(), (off / bound).max()

@@ -82,3 +82,9 @@ def test_attack_on_answers(host, name, monkeypatch):
 @pytest.mark.parametrize("rest,twice", [(False, False), (True, False), (False, True), (True, True)])
 def test_near_the_teacher(host, rest, twice):
     edges.check_near_the_teacher(rest, twice, "cpu")
+
+
+@pytest.mark.parametrize("spread", [1.0, 8.0])
+@pytest.mark.parametrize("dtype,pairs", [(edges.BF16, True), (edges.BF16, False), (edges.F16, True), (edges.F16, False)])
+def test_dq_of_few_heavy_keys(host, dtype, pairs, spread):
+    edges.check_dq_of_few_heavy_keys(dtype, pairs, spread, "cpu")

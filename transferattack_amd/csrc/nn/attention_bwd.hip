@@ -19,6 +19,7 @@ namespace ta_nn {
 template <class T, int DP, int BIASES>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_q(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = sizeof(T) == 2 ? 2 : kSubs<DP>, ROWS = 16 * SUBS;
+    constexpr int SUMS = sizeof(T) == 2 ? 2 : 1;         // of ds k, and of p k for the correction below
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
     T* vs = ks + ROWS * Tile<T, DP>::LD;
@@ -62,17 +63,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     const Column col = query_column(a, a.bias_in_lds ? bias_lds : nullptr, b, head, query, start, keys);
     const int64_t pos0 = static_cast<int64_t>(start) + i0, pos1 = static_cast<int64_t>(start) + min(i0 + 64, a.m) - 1;
 
-    // delta for this kernel is out . grad.  For 16-bit tensors out is rounded, and so were the probabilities it was made with; for
-    // the table, whose gradient is a sum of differences that nearly cancel, and for the keys it is taken anew: sum_j p_ij dp_ij.
-    // So it is for this kernel where a row is a single tile: with few keys out is as large as they are, and its rounding counts
-    // (over n keys it weighs a sqrt(n)-th of that of ds).
+    // delta while the keys pass is out . grad.  For 16-bit tensors out is rounded, and so were the probabilities it was made with; the
+    // exact one, sum_j p_ij dp_ij, is known at the end of the row (or at once, where the row is a single tile).  It is written for the
+    // other kernels, and what dq lacks is put right:  dq = sum ds k + (out . grad - delta) sum p k.  The second sum takes its operands
+    // from the fragments that the first has read.  Without it dq of bf16 rows whose mass lies on a few of 200 keys is 5 times as far
+    // off as its rounding.
     float exact = 0.0f;
     // sums past either end of the distances, for the table: of p and of p dp, since delta is not known yet
     float far_p[2] = {0.0f, 0.0f}, far_dp[2] = {0.0f, 0.0f};
     const bool wants_far = BIASES != kByPair && a.far != nullptr;
-    f32x4 dq[1][DT];
+    f32x4 dq[SUMS][DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = 0; x < SUMS; ++x)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dq[x][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const T* k_base = static_cast<const T*>(a.k) + b * a.k_sb + hk * a.k_sh;
     const T* v_base = static_cast<const T*>(a.v) + b * a.v_sb + hk * a.v_sh;
     Staged<T, DP, ROWS, 256> kr, vr;
@@ -90,7 +94,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
         const Kind kind = tile_kind<BIASES>(a, j0 + ROWS <= keys && (!a.causal || j0 + ROWS - 1 <= pos0), true, j0 - pos1 - a.first,
                                             j0 + ROWS - 1 - pos0 - a.first);
         if (busy) by_kind<BIASES>(kind, [&](auto tag) {
-        f32x4 s[SUBS], ds[1][SUBS];
+        f32x4 s[SUBS], ds[SUMS][SUBS];
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             s[t] = ds[0][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -114,7 +118,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
 #pragma unroll
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) ds[0][t][r] = s[t][r] * (ds[0][t][r] - delta);
+            for (int r = 0; r < 4; ++r) {
+                ds[0][t][r] = s[t][r] * (ds[0][t][r] - delta);
+                if constexpr (SUMS == 2) ds[1][t][r] = s[t][r];
+            }
         exact += exact_tile;
         if constexpr (BIASES != kByPair && decltype(tag)::kind != kNear) {
             const int64_t j64 = j0 & ~63;
@@ -131,10 +138,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
                 far_dp[1] += end > 0 ? exact_tile : 0.0f;
             }
         }
-        mma_transposed<DP, 1, SUBS>(ks, ds, dq, c, g);
+        mma_transposed<DP, SUMS, SUBS>(ks, ds, dq, c, g);
         });
     }
     exact = reduce_rows(exact, Sum{});
+    if constexpr (SUMS == 2) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) dq[0][dt] += dq[1][dt] * (delta - exact);
+    }
     if (valid && g == 0) a.delta[at] = exact;
     if (BIASES != kByPair && wants_far) {
         __shared__ float far_lds[4][2];
