@@ -359,3 +359,61 @@ def check_dq_of_few_heavy_keys(dtype, pairs, spread, device):
     x = attention_64(q, k, v, grad, table[index].movedim(-1, 0))
     off, bound = (dq.cpu().double() - x["dq"]).abs(), dq_bound(x, nn_oracle.half_step(dtype), 2.0 ** -25 if dtype == F16 else 0.0)
     assert (off <= bound).all(), (off / bound).max()
+
+
+def attention_gradients(x, plan, table, device, **options):
+    leaves = [t.to(device).requires_grad_(True) for t in (x["q"], x["k"], x["v"])]
+    out = relative_attention(*leaves, table.to(device), plan, **options)
+    return out, torch.autograd.grad(out, leaves, x["grad"].to(device))
+
+
+def check_range_of_fp16(n, size, pairs, device):
+    """gradients far from 1 and keys and queries that bring the results back into fp16's range: score gradients of `size` / n and less (below
+    2^-14, or past 65504) are rounded by half a step of fp16 like any others.  Bounds: dq_bound; dk likewise, with the exact delta"""
+    gen = torch.Generator().manual_seed(13)
+    m, dim, t = 40, 32, nn_oracle.half_step(F16)
+    q, k, v, grad = (torch.randn(1, 2, r, dim, generator=gen) for r in (m, n, n, m))
+    # products q.k stay of order 1 while one of the two takes a factor, dq = sum ds k and dk = sum ds q stay near 1
+    up = min(200.0, max(0.02, 10.0 / size))
+    table = torch.randn(5, 2, generator=gen)
+    if pairs:
+        index = torch.randint(0, 5, (m, n), generator=gen)
+        plan = RelativeBuckets.from_index(index.to(device))
+    else:
+        index = (torch.arange(n)[None] - torch.arange(m)[:, None] + 2).clamp(0, 4)
+        plan = RelativeBuckets.by_distance(torch.arange(5).to(device), -2)
+    for which in ("dq", "dk"):
+        qq, kk = (q / up, k * up) if which == "dq" else (q * up, k / up)
+        raw = {"q": qq.half(), "k": kk.half(), "v": (v * 30 if size > 1 else v).half(), "grad": (grad * size).half()}
+        assert all(r.isfinite().all() for r in raw.values())
+        out, grads = attention_gradients(raw, plan, table, device)
+        x = attention_64(raw["q"], raw["k"], raw["v"], raw["grad"], table[index].movedim(-1, 0))
+        got, want = dict(zip(("dq", "dk", "dv"), (g.cpu().double() for g in grads))), x
+        smallest = 2.0 ** -25
+        bounds = {"dq": dq_bound(x, t, smallest),
+                  "dk": (x["ds_err"] + (t + m * U) * x["ds"].abs()).transpose(-2, -1) @ x["q"].abs() * x["scale"] + (t + 2 * U) * x["dk"].abs() + smallest,
+                  "dv": (x["p"] * (x["rel"] + t + m * U)).transpose(-2, -1) @ x["grad"].abs() + t * x["dv"].abs() + smallest}
+        for name in (which, "dv"):
+            ok = want[name].abs() < 65504
+            off = (got[name] - want[name]).abs()
+            assert (off <= bounds[name])[ok].all(), (which, name, (off / bounds[name])[ok].max())
+
+
+def check_many_equal_keys(n, device):
+    """many equal probabilities below fp16's smallest normal number: their rounding, the same for all, would not average out.  Each is off
+    by half a step of fp16 as any number is, t, and the result by as much once more; n u of the sums"""
+    gen = torch.Generator().manual_seed(14)
+    dim, t = 8, nn_oracle.half_step(F16)
+    k, v = torch.zeros(1, 1, n, dim), (torch.rand(1, 1, n, dim, generator=gen) + 1.0).half()
+    k[0, 0, 0] = 1.0                                     # one key e^12.3 above the others: what they are compared with (76.3 steps of 2^-24)
+    plan = RelativeBuckets.from_index(torch.zeros(17, n, dtype=torch.int64).to(device))
+    for m in (1, 17):
+        q = torch.full((1, 1, m, dim), 12.3 * dim ** -0.5)
+        raw = {"q": q.half(), "k": k.half(), "v": v, "grad": torch.ones(1, 1, m, dim).half()}
+        here = plan if m == 17 else RelativeBuckets.from_index(torch.zeros(1, n, dtype=torch.int64).to(device))
+        out, grads = attention_gradients(raw, here, torch.zeros(1, 1), device)
+        x = attention_64(*(raw[r] for r in ("q", "k", "v", "grad")), torch.zeros(1, 1))
+        off = (out.detach().cpu().double() - x["out"]).abs()
+        assert (off <= (2 * t + (n + 400) * U) * x["out"]).all(), (off / x["out"]).max() / t
+        dv = grads[2].cpu().double()
+        assert ((dv - x["dv"]).abs() <= (2 * t + (n + 400) * U) * x["dv"] + 2.0 ** -25).all(), ((dv - x["dv"]).abs() / x["dv"]).max() / t

@@ -68,3 +68,15 @@ def test_near_the_teacher(rest, twice):
 @pytest.mark.parametrize("dtype,pairs", [(edges.BF16, True), (edges.BF16, False), (edges.F16, True), (edges.F16, False)])
 def test_dq_of_few_heavy_keys(dtype, pairs, spread):
     edges.check_dq_of_few_heavy_keys(dtype, pairs, spread, DEV)
+
+
+@pytest.mark.parametrize("pairs", [True, False])
+@pytest.mark.parametrize("size", [1e-6, 1e-4, 1e-2, 1e4])
+@pytest.mark.parametrize("n", [40, 200])
+def test_range_of_fp16(n, size, pairs):
+    edges.check_range_of_fp16(n, size, pairs, DEV)
+
+
+@pytest.mark.parametrize("n", [1000, 20000, 200000])
+def test_many_equal_keys(n):
+    edges.check_many_equal_keys(n, DEV)

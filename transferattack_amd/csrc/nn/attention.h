@@ -27,14 +27,17 @@ template <> struct Frag<float> {
     static constexpr int D = 16;                         // dims of a row fragment
     static constexpr int K = 16;                         // rows of a transposed fragment
     static constexpr int VE = 4;
+    static constexpr bool NARROW = false;
     typedef f32x4 Row;
 };
 template <> struct Frag<bf16> {
     static constexpr int D = 32, K = 32, VE = 8;
+    static constexpr bool NARROW = false;
     typedef bf16x8 Row;
 };
 template <> struct Frag<fp16> {
     static constexpr int D = 32, K = 32, VE = 8;
+    static constexpr bool NARROW = true;                 // the range of fp32 does not fit
     typedef half8 Row;
 };
 
@@ -110,6 +113,37 @@ __device__ __forceinline__ half8 pack8(f32x4 a, f32x4 b, fp16) {
     return half8{static_cast<_Float16>(a.x), static_cast<_Float16>(a.y), static_cast<_Float16>(a.z), static_cast<_Float16>(a.w),
                  static_cast<_Float16>(b.x), static_cast<_Float16>(b.y), static_cast<_Float16>(b.z), static_cast<_Float16>(b.w)};
 }
+// ---- fp16's range: 11 bits from 2^-14 up to 65504.  Probabilities are multiplied by 2^kLift before they are rounded (so down to 2^-26
+// of 1 keep their bits, and even scores that the passes make 2.7 apart do not overflow), score gradients, which may have any size, by a
+// power of two for each column that brings the largest so far to 2^11 .. 2^15.  All exact, and taken out of the sums again.
+template <class T> constexpr bool kNarrow = Frag<T>::NARROW;
+template <class T> constexpr int kLift = kNarrow<T> ? 12 : 0;
+template <int SUBS> __device__ __forceinline__ float peak_of(const f32x4 (&w)[SUBS]) {      // of a column, over its four lanes (NaN aside)
+    float peak = 0.0f;
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) peak = fmaxf(peak, fabsf(w[t][r]));
+    return reduce_rows(peak, [](float u, float v) { return fmaxf(u, v); });
+}
+__device__ __forceinline__ float lift_of(float peak) {   // 2^x with peak 2^x in [2^11, 2^12); 2^127 for the smallest
+    return __uint_as_float(static_cast<unsigned>(min(265 - static_cast<int>(__float_as_uint(peak) >> 23), 254)) << 23);
+}
+// w, a column's score gradients of one tile, times `up`; where that leaves the range, first `up` and the sums so far are made smaller
+template <int SUBS, int DT> __device__ __forceinline__ void into_range(f32x4 (&w)[SUBS], f32x4 (&sums)[DT], float& up) {
+    const float peak = peak_of(w);
+    const bool leaves = peak * up > 32768.0f;
+    if (wave_any(leaves)) {
+        const float to = leaves ? lift_of(peak) : up, by = to / up;
+        up = to;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) sums[dt] *= by;
+    }
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) w[t] *= up;
+}
+constexpr float kMostLift = 0x1p127f;                    // `up` before the first tile: any number that is not 0 leaves the range
+
 // ---- products that contract over a tile's rows
 // The weights of one column for 16 SUBS rows, as the matrix instructions take them: fp32 as they are; for 16-bit tensors
 // rounded to their type (an error of half a step per weight, independent from weight to weight, where the result itself is

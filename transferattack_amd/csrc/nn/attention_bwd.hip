@@ -5,8 +5,8 @@
 // Three kernels in the forward's form, each recomputing the scores: queries stay (dq, and delta for the others), keys stay
 // (dk, dv), and a tile of pairs stays while the batch streams past it (the table).  No sum crosses workgroups except the
 // table's, whose partial sums a last kernel adds in a fixed order.
-// p and ds are rounded to 16 bits where they enter a 16-bit matrix instruction: half a step of each term.  In fp16 terms below 2^-14
-// keep 2^-25 absolutely (p over more than some 10 000 equal keys, gradients below 6e-5: the same that their results are rounded by).
+// p and ds are rounded to 16 bits where they enter a 16-bit matrix instruction: half a step of each term (in fp16 brought into its
+// range before, see attention.h).
 // Together 9 products of m n dim, the forward's two aside, where 5 are needed: scores and dp are computed once for each kernel
 // rather than 16-bit sums exchanged through atomics, whose order would change results.  Bound like the forward by LDS reads and
 // issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 74 us, keys 87, table 42 + 20 (near tiles only: what is
@@ -69,6 +69,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     // from the fragments that the first has read.  Without it dq of bf16 rows whose mass lies on a few of 200 keys is 5 times as far
     // off as its rounding.
     float exact = 0.0f;
+    float up = kNarrow<T> ? kMostLift : 1.0f;
+    constexpr float LIFT = 1 << kLift<T>;
     // sums past either end of the distances, for the table: of p and of p dp, since delta is not known yet
     float far_p[2] = {0.0f, 0.0f}, far_dp[2] = {0.0f, 0.0f};
     const bool wants_far = BIASES != kByPair && a.far != nullptr;
@@ -120,8 +122,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 ds[0][t][r] = s[t][r] * (ds[0][t][r] - delta);
-                if constexpr (SUMS == 2) ds[1][t][r] = s[t][r];
+                if constexpr (SUMS == 2) ds[1][t][r] = s[t][r] * LIFT;
             }
+        if constexpr (kNarrow<T>) into_range(ds[0], dq[0], up);
         exact += exact_tile;
         if constexpr (BIASES != kByPair && decltype(tag)::kind != kNear) {
             const int64_t j64 = j0 & ~63;
@@ -144,7 +147,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     exact = reduce_rows(exact, Sum{});
     if constexpr (SUMS == 2) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) dq[0][dt] += dq[1][dt] * (delta - exact);
+        for (int dt = 0; dt < DT; ++dt) dq[0][dt] = dq[0][dt] * (1.0f / up) + dq[1][dt] * ((delta - exact) / LIFT);
     }
     if (valid && g == 0) a.delta[at] = exact;
     if (BIASES != kByPair && wants_far) {
@@ -195,6 +198,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     f32x4 dk[1][DT], dv[1][DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    float up = kNarrow<T> ? kMostLift : 1.0f;
+    constexpr float LIFT = 1 << kLift<T>;
 
     // the first query that sees any key of the block
     const int i_first = a.causal ? max(0, clamp_token(static_cast<int64_t>(j0) - start)) / ROWS * ROWS : 0;
@@ -256,10 +262,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float w = exp2_hw(p[0][t][r] - top[r]) * inv[r];
-                p[0][t][r] = w;
+                p[0][t][r] = w * LIFT;
                 ds[0][t][r] = w * (ds[0][t][r] - delta[r]);
             }
         }
+        if constexpr (kNarrow<T>) into_range(ds[0], dk[0], up);
         mma_transposed<DP, 1, SUBS>(gs, p, dv, c, g);
         mma_transposed<DP, 1, SUBS>(qs, ds, dk, c, g);
         });
@@ -269,8 +276,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
         for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if (valid) {
-        store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + static_cast<int64_t>(key) * a.dk_sn, dk[0], a.scale, a.dim, g);
-        store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + static_cast<int64_t>(key) * a.dv_sn, dv[0], 1.0f, a.dim, g);
+        store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + hk * a.dk_sh + static_cast<int64_t>(key) * a.dk_sn, dk[0], a.scale * (1.0f / up), a.dim, g);
+        store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + hk * a.dv_sh + static_cast<int64_t>(key) * a.dv_sn, dv[0], 1.0f / LIFT, a.dim, g);
     }
 }
 

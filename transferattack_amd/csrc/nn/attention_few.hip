@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
         for (int t = 0; t < SUBS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, s[0][t][r]);
-        top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); });
+        top = reduce_rows(top, [](float x, float y) { return fmaxf(x, y); }) - kLift<T>;      // (the reference: below the largest)
         const float m_new = fmaxf(m_run, top), m_ref = m_new == -INFINITY ? 0.0f : m_new;
         const float shrink = exp2_hw(m_run - m_ref);
         m_run = m_new;

@@ -4,6 +4,7 @@
 namespace ta_nn {
 
 constexpr float kSlack = 8.0f;
+template <class T> constexpr float kBelow = kNarrow<T> ? 15.0f - kSlack : 0.0f;      // how far below the largest score the reference is
 
 // One workgroup: 64 NQ columns (queries; those of all heads that share a key head in one row, so that shared heads share the
 // tiles) against every key they see, a tile at a time.  Two tiles in LDS: while one is worked on, the next arrives in registers
@@ -122,11 +123,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 3 : 2) void attent
                     for (int t = 0; t < SUBS; ++t)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) top[x] = fmaxf(top[x], s[x][t][r]);
-                    top[x] = reduce_rows(top[x], [](float u, float v) { return fmaxf(u, v); });
+                    top[x] = reduce_rows(top[x], [](float u, float v) { return fmaxf(u, v); }) - kBelow<T>;
                     more = more || top[x] > m_run[x] + kSlack;
                 }
-                // The reference is the largest score up to 2^kSlack: sums and outputs are rescaled only where one exceeds it by
-                // more, which after a few tiles is hardly ever.  (Probabilities up to 2^kSlack cost no precision.)
+                // The reference is the largest score up to 2^kSlack (fp16: and 2^7 below it, so that the many small probabilities of a
+                // long row keep their bits): sums and outputs are rescaled only where one exceeds it by more, which after a few tiles is
+                // hardly ever.  (Probabilities up to 2^kSlack cost no precision; they stay below 2^15.)
                 if (__ballot(more) != 0) {
 #pragma unroll
                     for (int x = 0; x < NQ; ++x) {

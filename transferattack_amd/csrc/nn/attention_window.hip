@@ -142,7 +142,10 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
     T* qs = vs + TILE;
     T* gs = qs + TILE;
     T* ps = gs + TILE;
-    T* dss = ps + 64 * WLD;
+    T* dss = ps + 64 * WLD;                              // fp16: in 32 bits, until the column's largest is known
+    constexpr int FLD = 64 + 4;
+    float* dss32 = reinterpret_cast<float*>(dss);
+    constexpr float LIFT = 1 << kLift<T>;
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const Share share(a, parts);
     const int own = 16 * wave + c;                       // this lane's query, and later its key
@@ -209,17 +212,20 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
                     const float w = p[t][r];
                     ds[0][t][r] = w * (ds[0][t][r] - delta);
                     table_sum[t][r] += ds[0][t][r];
-                    ps[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(w);
-                    dss[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(ds[0][t][r]);
+                    ps[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(w * LIFT);
+                    if constexpr (kNarrow<T>) dss32[(16 * t + 4 * g + r) * FLD + own] = ds[0][t][r];
+                    else dss[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(ds[0][t][r]);
                 }
         }
         {
             f32x4 dq[1][DT];
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            float up = kNarrow<T> ? kMostLift : 1.0f;
+            if constexpr (kNarrow<T>) into_range(ds[0], dq[0], up);
             mma_transposed<DP, 1, 4>(ks, ds, dq, c, g);
             if (own < a.m)
-                store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + share.head * a.dq_sh + own * a.dq_sm, dq[0], a.scale, a.dim, g);
+                store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + share.head * a.dq_sh + own * a.dq_sm, dq[0], a.scale * (1.0f / up), a.dim, g);
         }
         __syncthreads();
         {
@@ -229,11 +235,20 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
             for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             w[0].from_lds(ps + own * WLD, g);
             mma_transposed<DP, 1, 4>(gs, w, dv, c, g);
-            w[0].from_lds(dss + own * WLD, g);
+            float up = kNarrow<T> ? kMostLift : 1.0f;
+            if constexpr (kNarrow<T>) {
+                f32x4 column[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) column[t] = *reinterpret_cast<const f32x4*>(dss32 + own * FLD + 16 * t + 4 * g);
+                into_range(column, dk[0], up);
+                w[0].from_tiles(column);
+            } else {
+                w[0].from_lds(dss + own * WLD, g);
+            }
             mma_transposed<DP, 1, 4>(qs, w, dk, c, g);
             if (own < a.n) {
-                store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + share.head * a.dk_sh + own * a.dk_sn, dk[0], a.scale, a.dim, g);
-                store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + share.head * a.dv_sh + own * a.dv_sn, dv[0], 1.0f, a.dim, g);
+                store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + share.head * a.dk_sh + own * a.dk_sn, dk[0], a.scale * (1.0f / up), a.dim, g);
+                store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + share.head * a.dv_sh + own * a.dv_sn, dv[0], 1.0f / LIFT, a.dim, g);
             }
         }
         __syncthreads();                                 // the tiles are free
@@ -263,7 +278,8 @@ template <class T, int DP> int launch_window_by(AttentionArgs a, bool backward, 
         hipLaunchKernelGGL((window_fwd<T, DP>), dim3(static_cast<unsigned>(blocks)), dim3(256), 4 * tile, st, a, parts);
         return check_launch("ta_nn_attention");
     }
-    const size_t lds = 4 * tile + 2 * 64 * (64 + 16 / sizeof(T)) * sizeof(T), diagonals = 64 * 65 * 4;
+    const size_t weights = 64 * (64 + 16 / sizeof(T)) * sizeof(T), diagonals = 64 * 65 * 4;
+    const size_t lds = 4 * tile + weights + (kNarrow<T> ? 64 * (64 + 4) * 4 : weights);
     hipLaunchKernelGGL((window_bwd<T, DP>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds > diagonals ? lds : diagonals, st, a, parts);
     return check_launch("ta_nn_attention_backward");
 }
