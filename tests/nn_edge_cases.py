@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import nn_oracle
-from nn_cases import BF16, F16, F32  # noqa: F401
+from nn_cases import BF16, F16, F32, case, check_attention, make_attention  # noqa: F401
 from transferattack_amd.distill import TopLogits, distillation_loss, distillation_loss_and_grad, top_logits
 from transferattack_amd.relative import RelativeBuckets, relative_attention, relative_attention_packed
 
@@ -417,3 +417,100 @@ def check_many_equal_keys(n, device):
         assert (off <= (2 * t + (n + 400) * U) * x["out"]).all(), (off / x["out"]).max() / t
         dv = grads[2].cpu().double()
         assert ((dv - x["dv"]).abs() <= (2 * t + (n + 400) * U) * x["dv"] + 2.0 ** -25).all(), ((dv - x["dv"]).abs() / x["dv"]).max() / t
+
+
+# ---- loops that go round more than once, and kernels that small cases do not reach
+MANY = {
+    "windows, five to a workgroup": case(m=5, batch=900, heads=4, dim=32),
+    "windows in turn, bf16": case(m=9, batch=900, heads=4, dim=64, dtype=BF16),
+    "windows with masks, two to a workgroup": case(m=16, batch=512, heads=8, dim=32, mask="windows"),
+    "windows with masks, fp16": case(m=16, batch=512, heads=8, dim=32, mask="windows", dtype=F16),
+    "windows by distance": case(m=7, n=12, batch=900, heads=4, pairs=False, causal=True, start=4),
+    "table of distances": case(m=70, batch=300, heads=2, pairs=False, lengths=[(29 * i) % 71 for i in range(300)], dtype=BF16),
+    "table of distances fp32": case(m=66, batch=300, heads=2, pairs=False, causal=True),
+    "table of pairs": case(m=66, n=67, batch=256, heads=2, dtype=BF16, dim=64),
+    "table of pairs, masked": case(m=66, n=67, batch=256, heads=2, dtype=F16, dim=64, mask="key"),
+    "table of pairs, lengths": case(m=66, n=67, batch=256, heads=2, dtype=F16, lengths=[(31 * i) % 68 for i in range(256)]),
+}
+WIDE = ("table of pairs", "table of pairs, masked", "table of pairs, lengths")       # 32 queries to a wave, too: 16-bit pairs, 512 workgroups
+
+
+def sequences_of_a_workgroup(c):
+    """how many sequences share a part of the table's sums, from the workspace that the library asks for"""
+    from transferattack_amd import _nn
+    a = _nn.AttentionArgs()
+    heads, m, n, batch = c["heads"], c["m"], c["n"] or c["m"], c["batch"]
+    a.dtype, a.batch, a.heads, a.kv_heads, a.m, a.n, a.dim = _nn.DTYPES[c["dtype"]], batch, heads, c["kv"] or heads, m, n, c["dim"]
+    a.buckets, a.distances, a.start, a.causal, a.dtable = c["buckets"], 0 if c["pairs"] else 14, c["start"], int(c["causal"]), 1
+    a.first = -6
+    if c["mask"] == "windows":
+        a.mask_kind, a.mask_period = _nn.MASK_FLOAT, batch // 2
+    elif c["mask"] == "key":
+        a.mask_kind, a.mask_period = _nn.MASK_BOOL, 1
+    a.key_lengths = None if c["lengths"] is None else 1
+    floats = _nn.load().ta_nn_attention_workspace(a, 1) - batch * heads * m
+    q_tiles, k_tiles = -(-m // 64), -(-n // 64)
+    if c["pairs"]:
+        return batch * m * n * heads / floats
+    floats -= batch * heads * q_tiles * 2 + heads * (q_tiles + k_tiles - 1) * 128
+    return batch * q_tiles * min(k_tiles, 3) * 128 * heads / floats
+
+
+def check_many(name, device):
+    c = MANY[name]
+    assert sequences_of_a_workgroup(c) >= 2, sequences_of_a_workgroup(c)
+    check_attention(c, device)
+
+
+OTHER_BIASES = {
+    "distances, bool mask": case(m=70, n=75, pairs=False, mask="bool", dtype=BF16),
+    "distances, mask of heads": case(m=70, n=75, pairs=False, mask="heads", causal=True, lengths=[75, 40], kv=1),
+    "distances, additive masks": case(m=66, n=66, pairs=False, mask="windows", batch=4, dtype=F16, dim=64),
+    "distances, mask of infinities": case(m=40, n=70, pairs=False, mask="infinite", start=30),
+    "few queries, distances, mask": case(m=2, n=90, pairs=False, mask="bool", kv=1, heads=4, start=60),
+    "large table of pairs": case(m=66, n=70, buckets=7000, dtype=BF16),
+}
+
+
+def check_many_distances(dtype, m, n, causal, device):
+    """a line of 9000 distances, each its own bucket for the most part: more than the kernels keep on the chip, so the table is read where it is"""
+    gen = torch.Generator().manual_seed(16)
+    batch, heads, dim, start = 2, 2, 32, n - m
+    q, k, v, grad = (torch.randn(batch, heads, t, dim, generator=gen).to(dtype) for t in (m, n, n, m))
+    line = torch.arange(9000) % 8500
+    table = torch.randn(8500, heads, generator=gen)
+    distance = torch.arange(n)[None] - torch.arange(m)[:, None] - start
+    bucket = line[(distance + 4500).clamp(0, 8999)][None]
+    allowed = (distance <= 0).expand(batch, heads, m, n) if causal else None
+    want = nn_oracle.attention(q, k, v, table, bucket, dim ** -0.5, allowed, None, grad, dtype)
+    leaves = [t.to(device).requires_grad_(True) for t in (q, k, v, table)]
+    plan = RelativeBuckets.by_distance(line.to(device), -4500)
+    out = relative_attention(*leaves, plan, causal=causal, query_start=start)
+    nn_oracle.close("out", out, want["out"])
+    # (a result below 2^-14 is rounded by half a step of fp16's smallest numbers, 2^-25, not by a share of itself as the oracle counts)
+    smallest = 2.0 ** -25 if dtype == F16 else 0.0
+    for name, got in zip(("dq", "dk", "dv", "dtable"), torch.autograd.grad(out, leaves, grad.to(device))):
+        nn_oracle.close(name, got, (want[name][0], want[name][1] + (0.0 if name == "dtable" else smallest)), F32 if name == "dtable" else None)
+
+
+def check_frozen_table(c, device):
+    """a frozen surrogate: gradients of what it is given, none of its table -- the bits of the call that has both, packed and not"""
+    x, plan, options, _ = make_attention(c, device)
+    leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v")]
+    alone = torch.autograd.grad(relative_attention(*leaves, x["table"], plan, **options), leaves, x["grad"])
+    table = x["table"].clone().requires_grad_(True)
+    both = torch.autograd.grad(relative_attention(*leaves, table, plan, **options), leaves + [table], x["grad"])
+    assert all(torch.equal(a, b) for a, b in zip(alone, both))
+    (only,) = torch.autograd.grad(relative_attention(*[t.detach() for t in leaves], table, plan, **options), table, x["grad"])
+    assert torch.equal(only, both[3])
+    options.pop("query_start")
+    qkv = torch.stack([t.detach() for t in leaves]).permute(1, 3, 0, 2, 4).contiguous().requires_grad_(True)
+    (dqkv,) = torch.autograd.grad(relative_attention_packed(qkv, x["table"], plan, **options), qkv, x["grad"].transpose(1, 2).flatten(2))
+    assert all(torch.equal(dqkv[:, :, i].transpose(1, 2), alone[i]) for i in range(3))
+
+
+FROZEN = {
+    "windows": case(m=49, batch=6, heads=3, dim=32, mask="windows"),
+    "pairs bf16": case(m=70, batch=2, dim=64, dtype=BF16),
+    "distances fp16": case(m=70, batch=2, pairs=False, causal=True, dtype=F16),
+}

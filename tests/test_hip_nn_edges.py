@@ -1,5 +1,6 @@
 """nn_edge_cases on the GPU (libta_nn.so)."""
 import pytest
+import torch
 
 import nn_edge_cases as edges
 import transferattack_amd
@@ -80,3 +81,37 @@ def test_range_of_fp16(n, size, pairs):
 @pytest.mark.parametrize("n", [1000, 20000, 200000])
 def test_many_equal_keys(n):
     edges.check_many_equal_keys(n, DEV)
+
+
+@pytest.mark.parametrize("name", sorted(edges.MANY))
+def test_many(name):
+    edges.check_many(name, DEV)
+
+
+@pytest.mark.parametrize("name", sorted(edges.OTHER_BIASES))
+def test_other_biases(name):
+    edges.check_attention(edges.OTHER_BIASES[name], DEV)
+
+
+@pytest.mark.parametrize("dtype,m,n,causal", [(edges.F32, 70, 75, False), (edges.BF16, 70, 80, True), (edges.F16, 3, 90, True)])
+def test_many_distances(dtype, m, n, causal):
+    edges.check_many_distances(dtype, m, n, causal, DEV)
+
+
+@pytest.mark.parametrize("name", sorted(edges.FROZEN))
+def test_frozen_table(name):
+    edges.check_frozen_table(edges.FROZEN[name], DEV)
+
+
+def test_paths_of_the_cases():
+    """the kernels that the cases above are there for are those that run: read from a trace"""
+    names = set()
+    for name in ("table of pairs", "table of pairs, masked", "windows with masks, two to a workgroup", "table of distances"):
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as trace:
+            edges.check_attention(edges.MANY[name], DEV)
+            torch.cuda.synchronize()
+        names |= {e.name for e in trace.events()}
+    print(sorted(n[:80] for n in names if "attention" in n or "window" in n))
+    for want in ("attention_fwd<ta_nn::bf16, 64, 2, 1>", "attention_fwd<ta_nn::fp16, 64, 2, 2>", "window_fwd<float, 32>", "window_bwd<float, 32>",
+                 "attention_bwd_table<ta_nn::bf16, 32, 0>", "attention_distance_sums"):
+        assert any(want in n for n in names), (want, sorted(names))

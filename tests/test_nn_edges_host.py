@@ -100,3 +100,23 @@ def test_range_of_fp16(host, n, size, pairs):
 @pytest.mark.parametrize("n", [20000])
 def test_many_equal_keys(host, n):
     edges.check_many_equal_keys(n, "cpu")
+
+
+@pytest.mark.parametrize("name", ["windows, five to a workgroup", "table of distances", "table of pairs, masked"])      # (the others: 1 to 50 s each here)
+def test_many(host, name):
+    edges.check_many(name, "cpu")
+
+
+@pytest.mark.parametrize("name", sorted(edges.OTHER_BIASES))
+def test_other_biases(host, name):
+    edges.check_attention(edges.OTHER_BIASES[name], "cpu")
+
+
+@pytest.mark.parametrize("dtype,m,n,causal", [(edges.F32, 70, 75, False), (edges.BF16, 70, 80, True), (edges.F16, 3, 90, True)])
+def test_many_distances(host, dtype, m, n, causal):
+    edges.check_many_distances(dtype, m, n, causal, "cpu")
+
+
+@pytest.mark.parametrize("name", sorted(edges.FROZEN))
+def test_frozen_table(host, name):
+    edges.check_frozen_table(edges.FROZEN[name], "cpu")
