@@ -81,6 +81,8 @@ typedef struct ta_nn_attention_args {
     const int32_t* pair_starts;                  /*        [buckets + 1] where each bucket begins among them */
 } ta_nn_attention_args;
 
+/* floats of workspace the call needs (pointers of args need not be set yet, but dtable has to be NULL or not); 0: none, or
+ * sizes that the call refuses */
 int64_t ta_nn_attention_workspace(const ta_nn_attention_args* args, int backward);
 int ta_nn_attention(const ta_nn_attention_args* args, void* stream);
 int ta_nn_attention_backward(const ta_nn_attention_args* args, void* stream);

@@ -120,3 +120,25 @@ def test_many_distances(host, dtype, m, n, causal):
 @pytest.mark.parametrize("name", sorted(edges.FROZEN))
 def test_frozen_table(host, name):
     edges.check_frozen_table(edges.FROZEN[name], "cpu")
+
+
+def test_workspace_of_bad_sizes():
+    """the C entry that sizes the workspace is asked before the call checks anything: it answers 0, it does not divide by them"""
+    from transferattack_amd import _nn
+    good = dict(dtype=1, batch=3, heads=4, kv_heads=2, m=70, n=80, dim=32, buckets=5, distances=5, dtable=1)
+
+    def floats(lib, backward, **change):
+        a = _nn.AttentionArgs()
+        for field, value in dict(good, **change).items():
+            setattr(a, field, value)
+        return lib.ta_nn_attention_workspace(a, backward)
+
+    lib = _nn.load()
+    assert floats(lib, 1) > 0 and floats(lib, 1, dtable=None) == 3 * 4 * 70
+    low = -(1 << 31)
+    for change in (dict(mask_kind=1, mask_period=0), dict(mask_kind=2, mask_period=-3), dict(mask_kind=9), dict(heads=0), dict(heads=3), dict(heads=low),
+                   dict(kv_heads=0), dict(batch=0), dict(batch=low), dict(m=low), dict(n=0), dict(dim=0), dict(dim=200), dict(distances=-1),
+                   dict(distances=low), dict(buckets=0), dict(dtype=7), dict(table_dtype=-1), dict(m=1 << 30), dict(q_sm=-1)):
+        for backward in (0, 1):
+            for size in ({}, dict(m=5, n=5)):
+                assert floats(lib, backward, **dict(size, **change)) == 0, change
