@@ -89,7 +89,7 @@ int ta_nn_attention_backward(const ta_nn_attention_args* args, void* stream);
 
 /* ---- a teacher's top logits -------------------------------------------------------------------------------------------
  * values / top_classes [rows][k]: the k largest of each row in falling order, equal ones by the lowest class (NaN above all);
- * rest [rows] (or NULL): log sum exp(x / temperature) over the other classes, -inf if there are none. */
+ * rest [rows] (or NULL): log sum exp(x / temperature) over the other classes, -inf if there are none.  At most 2^30 classes. */
 int ta_nn_top_logits(const void* x, int dtype, int64_t x_stride, int64_t rows, int classes, int k, float temperature, float* values,
                      int64_t* top_classes, float* rest, void* stream);
 

@@ -142,3 +142,27 @@ def test_workspace_of_bad_sizes():
         for backward in (0, 1):
             for size in ({}, dict(m=5, n=5)):
                 assert floats(lib, backward, **dict(size, **change)) == 0, change
+
+
+def test_sizes_past_32_bits(host):
+    """tensors expanded to more than the library's sizes hold are refused, not cut to their lower 32 bits"""
+    import torch
+    from transferattack_amd.distill import TopLogits, distillation_loss, top_logits
+    from transferattack_amd.relative import RelativeBuckets, relative_attention, relative_attention_packed
+    many = (1 << 32) + 7
+    line, table, q = RelativeBuckets.by_distance(torch.arange(5), -2), torch.zeros(5, 1), torch.randn(1, 1, 3, 8)
+    long = torch.randn(1, 1, 1, 8).expand(1, 1, many, 8)
+    for call in (lambda: relative_attention(q, long, long, table, line), lambda: relative_attention(long, q, q, table, line),
+                 lambda: relative_attention(q.expand(many, 1, 3, 8), q.expand(many, 1, 3, 8), q.expand(many, 1, 3, 8), table, line),
+                 lambda: relative_attention_packed(torch.randn(1, 1, 3, 1, 8).expand(1, many, 3, 1, 8), table, line)):
+        with pytest.raises(ValueError, match="2.30"):
+            call()
+    x = torch.zeros(1, 1)
+    for call in (lambda: top_logits(x.expand(1, many), 3), lambda: top_logits(x.expand(1, (1 << 30) + 1), 3),
+                 lambda: distillation_loss(x.expand(1, many), TopLogits(torch.zeros(1, 1), torch.zeros(1, 1, dtype=torch.int64)))):
+        with pytest.raises(ValueError, match="classes"):
+            call()
+    from transferattack_amd import _nn
+    at = x.data_ptr()                                    # the C entry, whose sizes are 32-bit already
+    assert _nn._lib.ta_nn_top_logits(at, 0, 1 << 31, 1, (1 << 31) - 1, 1, 1.0, at, at, None, None) == -1
+    assert b"2^30" in _nn._lib.ta_nn_last_error()

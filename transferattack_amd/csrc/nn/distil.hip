@@ -740,7 +740,9 @@ extern "C" int ta_nn_top_logits(const void* x, int dtype, int64_t x_stride, int6
                                 float* values, int64_t* top_classes, float* rest, void* stream) {
     TA_NN_REQUIRE(x && values && top_classes, "null pointer");
     TA_NN_REQUIRE(rows >= 1 && rows <= 0x7FFFFFFF, "rows %lld", static_cast<long long>(rows));
-    TA_NN_REQUIRE(classes >= 1 && x_stride >= classes, "%d classes, row stride %lld", classes, static_cast<long long>(x_stride));
+    // (a thread's place in its last pass lies up to 8192 elements behind the row)
+    TA_NN_REQUIRE(classes >= 1 && classes <= (1 << 30) && x_stride >= classes, "%d classes (1 .. 2^30), row stride %lld", classes,
+                  static_cast<long long>(x_stride));
     TA_NN_REQUIRE(k >= 1 && k <= classes && k <= ta_nn::kMaxTop, "%d of %d classes (at most %d)", k, classes, ta_nn::kMaxTop);
     TA_NN_REQUIRE(temperature > 0.0f && temperature < INFINITY, "temperature %g", static_cast<double>(temperature));
     const ta_nn::TopArgs a{x, x_stride, classes, k, temperature, values, top_classes, rest};

@@ -19,7 +19,8 @@ from . import _nn
 
 FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 MAX_TOP = 1024
-MAX_CLASSES = 458752
+MAX_CLASSES = 458752                                     # of a student's row
+MAX_ROW = 1 << 30                                        # of a teacher's
 STATS = 5
 
 
@@ -79,6 +80,8 @@ def _rows_of(logits, name="logits"):
     _nn.check_tensor(logits, name, None, FLOATS)
     if logits.dim() < 1 or not 1 <= logits.shape[-1]:
         raise ValueError("%s must be [..., classes], got %s" % (name, tuple(logits.shape)))
+    if logits.shape[-1] > MAX_ROW:
+        raise ValueError("%d classes (at most %d)" % (logits.shape[-1], MAX_ROW))
     rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     if rows.stride(1) != 1 and rows.shape[1] > 1 or rows.stride(0) < rows.shape[1] and rows.shape[0] > 1:
         rows = rows.contiguous()

@@ -135,6 +135,8 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
         raise TypeError("buckets must be RelativeBuckets, got %s" % type(buckets).__name__)
     batch, heads, m, dim = q.shape
     n = k.shape[2]
+    if max(batch, heads, m, n) >= 1 << 30:               # (an expanded tensor may be that long; the library's sizes have 32 bits)
+        raise ValueError("batch %d, %d heads, %d queries, %d keys (below 2^30 each)" % (batch, heads, m, n))
     _nn.check_tensor(table, "table", q, FLOATS)
     if table.dim() != 2 or table.shape[1] != heads:
         raise ValueError("table must be [buckets, %d heads], got %s" % (heads, tuple(table.shape)))
