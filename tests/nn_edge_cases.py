@@ -514,3 +514,13 @@ FROZEN = {
     "pairs bf16": case(m=70, batch=2, dim=64, dtype=BF16),
     "distances fp16": case(m=70, batch=2, pairs=False, causal=True, dtype=F16),
 }
+
+
+def check_no_rows(device):
+    """a batch of no rows has the shape of one, and gradients"""
+    x = torch.randn(0, 3, 9, device=device, requires_grad=True)
+    answers = top_logits(x, 2)
+    loss = distillation_loss(x, answers, reduction="none")
+    assert loss.shape == (0, 3) and torch.autograd.grad(loss.sum(), x)[0].shape == x.shape
+    for reduction in ("mean", "sum"):
+        assert distillation_loss(x, answers, reduction=reduction).shape == () and distillation_loss_and_grad(x, answers, reduction=reduction)[1].shape == x.shape

@@ -115,3 +115,7 @@ def test_paths_of_the_cases():
     for want in ("attention_fwd<ta_nn::bf16, 64, 2, 1>", "attention_fwd<ta_nn::fp16, 64, 2, 2>", "window_fwd<float, 32>", "window_bwd<float, 32>",
                  "attention_bwd_table<ta_nn::bf16, 32, 0>", "attention_distance_sums"):
         assert any(want in n for n in names), (want, sorted(names))
+
+
+def test_no_rows():
+    edges.check_no_rows(DEV)

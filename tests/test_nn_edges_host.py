@@ -166,3 +166,7 @@ def test_sizes_past_32_bits(host):
     at = x.data_ptr()                                    # the C entry, whose sizes are 32-bit already
     assert _nn._lib.ta_nn_top_logits(at, 0, 1 << 31, 1, (1 << 31) - 1, 1, 1.0, at, at, None, None) == -1
     assert b"2^30" in _nn._lib.ta_nn_last_error()
+
+
+def test_no_rows(host):
+    edges.check_no_rows("cpu")

@@ -191,7 +191,7 @@ def distillation_loss(logits, answers, weight=None, reduction="mean"):
     rows = _rows_of(logits)
     o = _checked(rows, answers, weight, reduction)
     if rows.shape[0] == 0:
-        return rows.float().sum(dim=1) if reduction == "none" else rows.float().sum()
+        return rows.float().sum(dim=1).view(logits.shape[:-1]) if reduction == "none" else rows.float().sum()
     if torch.is_grad_enabled() and rows.requires_grad:
         loss = _Distillation.apply(rows, o)
     else:
