@@ -524,3 +524,19 @@ def check_no_rows(device):
     assert loss.shape == (0, 3) and torch.autograd.grad(loss.sum(), x)[0].shape == x.shape
     for reduction in ("mean", "sum"):
         assert distillation_loss(x, answers, reduction=reduction).shape == () and distillation_loss_and_grad(x, answers, reduction=reduction)[1].shape == x.shape
+
+
+def check_plan_keeps_its_buckets(device):
+    """a plan never changes: not with the tensor it was made from, nor does its copy on another device"""
+    index, line = torch.arange(12).view(3, 4).to(device), torch.arange(5).to(device)
+    plans = RelativeBuckets.from_index(index), RelativeBuckets.by_distance(line, -2)
+    q, k = torch.randn(1, 2, 3, 8, device=device), torch.randn(1, 2, 4, 8, device=device)
+    table = torch.randn(12, 2, device=device)
+    before = [relative_attention(q, k, k, table, p) for p in plans]
+    index.zero_(), line.zero_()
+    other = "cpu:0" if device == "cpu" else "cpu"        # (another device than "cpu" by name: made anew)
+    for p, want in zip(plans, before):
+        moved = p.to(other)
+        assert torch.equal(moved.source.cpu(), torch.arange(12).view(3, 4) if p.shape else torch.arange(5))
+        assert torch.equal(relative_attention(q, k, k, table, p), want)
+        assert torch.equal(relative_attention(q, k, k, table, moved.to(device)), want)

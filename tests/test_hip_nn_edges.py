@@ -119,3 +119,7 @@ def test_paths_of_the_cases():
 
 def test_no_rows():
     edges.check_no_rows(DEV)
+
+
+def test_plan_keeps_its_buckets():
+    edges.check_plan_keeps_its_buckets(DEV)

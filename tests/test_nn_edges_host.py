@@ -170,3 +170,7 @@ def test_sizes_past_32_bits(host):
 
 def test_no_rows(host):
     edges.check_no_rows("cpu")
+
+
+def test_plan_keeps_its_buckets(host):
+    edges.check_plan_keeps_its_buckets("cpu")

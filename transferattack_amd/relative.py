@@ -57,7 +57,7 @@ class RelativeBuckets:
         order = torch.sort(flat, stable=True)[1].to(torch.int32)
         starts = torch.zeros(buckets + 1, dtype=torch.int64, device=index.device)
         starts[1:] = torch.cumsum(torch.bincount(flat, minlength=buckets), 0)
-        return cls._new(source=index, device=index.device, buckets=buckets, shape=(m, n), distances=0, first=0, index=padded(index),
+        return cls._new(source=index.detach().clone(), device=index.device, buckets=buckets, shape=(m, n), distances=0, first=0, index=padded(index),
                         index_t=padded(index.t()), order=order, starts=starts.to(torch.int32))
 
     @classmethod
@@ -68,7 +68,7 @@ class RelativeBuckets:
         low, high = int(buckets.min()), int(buckets.max())
         if low < 0 or high > 65535:
             raise ValueError("bucket numbers must be 0 .. 65535, got %d .. %d" % (low, high))
-        return cls._new(source=buckets, device=buckets.device, buckets=high + 1, shape=None, distances=buckets.numel(), first=first,
+        return cls._new(source=buckets.detach().clone(), device=buckets.device, buckets=high + 1, shape=None, distances=buckets.numel(), first=first,
                         index=buckets.to(torch.int32).contiguous().clone(), index_t=None, order=None, starts=None)
 
     @classmethod
