@@ -123,3 +123,16 @@ def test_no_rows():
 
 def test_plan_keeps_its_buckets():
     edges.check_plan_keeps_its_buckets(DEV)
+
+
+def test_plan_on_other_streams():
+    """a plan made on one stream is ready for all: nothing of its making is still under way, and calls elsewhere see it whole"""
+    side = torch.cuda.Stream()
+    index = torch.randint(0, 5000, (2100, 2100), generator=torch.Generator().manual_seed(0)).to(DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        plan = edges.RelativeBuckets.from_index(index)
+        assert side.query()
+        line = edges.RelativeBuckets.by_distance(torch.arange(100000, device=DEV) % 7, -5)
+        assert side.query()
+    assert torch.equal(plan.order, torch.sort(index.flatten(), stable=True)[1].int()) and torch.equal(line.index.cpu(), (torch.arange(100000) % 7).int())

@@ -37,6 +37,8 @@ class RelativeBuckets:
     def _new(cls, **fields):
         self = object.__new__(cls)
         self.__dict__.update(fields)
+        if self.device.type == "cuda":                   # ready for every stream: a module keeps its plan from the first call on
+            torch.cuda.current_stream(self.device).synchronize()
         return self
 
     @classmethod
