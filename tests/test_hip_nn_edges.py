@@ -136,3 +136,17 @@ def test_plan_on_other_streams():
         line = edges.RelativeBuckets.by_distance(torch.arange(100000, device=DEV) % 7, -5)
         assert side.query()
     assert torch.equal(plan.order, torch.sort(index.flatten(), stable=True)[1].int()) and torch.equal(line.index.cpu(), (torch.arange(100000) % 7).int())
+
+
+def test_window_transformer_made_in_inference_mode(monkeypatch):
+    from transferattack_amd.backbones.timm_victims import WindowAttention
+    monkeypatch.setenv("TA_RELATIVE_ATTENTION", "1")
+    torch.manual_seed(0)
+    with torch.inference_mode():
+        layer = WindowAttention(32, 4, 2).to(DEV)
+        x = torch.randn(6, 16, 32, device=DEV)
+        got = layer(x)
+        monkeypatch.setenv("TA_RELATIVE_ATTENTION", "0")
+        want = layer(x)
+    # both sum some 100 products in 32 bits, in another order
+    assert (got - want).abs().max() <= 200 * edges.U * want.abs().max()

@@ -174,3 +174,17 @@ def test_no_rows(host):
 
 def test_plan_keeps_its_buckets(host):
     edges.check_plan_keeps_its_buckets("cpu")
+
+
+def test_plan_of_a_window_transformer():
+    """built once, again when a checkpoint replaces the index, and for models made in inference mode, whose tensors have no version"""
+    import torch
+    from transferattack_amd.backbones.timm_victims import WindowAttention
+    for made in (torch.no_grad, torch.inference_mode):
+        with made():
+            layer = WindowAttention(32, 4, 2)
+        plan = layer._buckets()
+        assert layer._buckets() is plan and plan.shape == (16, 16)
+        if made is torch.no_grad:
+            layer.load_state_dict(layer.state_dict())
+            assert layer._buckets() is not plan

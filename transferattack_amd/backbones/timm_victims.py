@@ -227,9 +227,10 @@ class WindowAttention(nn.Module):
     def _buckets(self):
         """the plan of ``relative_position_index``, built once per device (and again if a checkpoint replaces the index)"""
         index = self.relative_position_index
+        version = None if index.is_inference() else index._version       # (nothing counts the changes of a tensor made in inference mode)
         kept = self.__dict__.get("_ta_buckets")
-        if kept is None or kept[0] is not index or kept[1] != index._version:
-            kept = self.__dict__["_ta_buckets"] = (index, index._version, relative.RelativeBuckets.from_index(index))
+        if kept is None or kept[0] is not index or kept[1] != version:
+            kept = self.__dict__["_ta_buckets"] = (index, version, relative.RelativeBuckets.from_index(index))
         return kept[2]
 
     def forward(self, x, mask=None):
