@@ -329,13 +329,14 @@ def attention_64(q, k, v, grad, bias):
                 dq=ds @ k * scale, dk=ds.transpose(-2, -1) @ q * scale, dv=p.transpose(-2, -1) @ grad)
 
 
-def dq_bound(x, t, smallest=0.0):
+def dq_bound(x, t, smallest=0.0, of_terms=None):
     """of dq where ds is rounded once (t of it) and delta is sum p dp: the delta that ds is formed with is out . grad, off by what out is
     rounded by twice (its probabilities, itself); put right it leaves that times t, of ds and of p.  `smallest`: half a step of the
-    type's smallest numbers, for the result"""
+    type's smallest numbers, for the result; `of_terms`: what ds is rounded by, if not t"""
+    of_terms = t if of_terms is None else of_terms
     out_err = (x["p"] * (x["rel"] + t + x["n"] * U)) @ x["v"].abs() + t * x["out"].abs()
     apart = (out_err * x["grad"].abs()).sum(-1, keepdim=True) + (x["dim"] + 4) * U * (x["out"] * x["grad"]).abs().sum(-1, keepdim=True)
-    terms = x["ds_err"] + (t + x["n"] * U) * x["ds"].abs() + (2 * t + x["n"] * U) * x["p"] * apart
+    terms = x["ds_err"] + (of_terms + x["n"] * U) * x["ds"].abs() + (2 * t + x["n"] * U) * x["p"] * apart
     return terms @ x["k"].abs() * x["scale"] + (t + 2 * U) * x["dq"].abs() + smallest
 
 
@@ -540,3 +541,49 @@ def check_plan_keeps_its_buckets(device):
         assert torch.equal(moved.source.cpu(), torch.arange(12).view(3, 4) if p.shape else torch.arange(5))
         assert torch.equal(relative_attention(q, k, k, table, p), want)
         assert torch.equal(relative_attention(q, k, k, table, moved.to(device)), want)
+
+
+SHORT = [(BF16, 5, 5, 3, 3, 32), (F16, 4, 4, 3, 3, 64), (BF16, 49, 49, 2, 2, 32), (F16, 64, 64, 2, 2, 64), (F16, 3, 9, 2, 2, 40),      # windows
+         (BF16, 20, 30, 4, 2, 32), (F16, 2, 2, 4, 4, 128), (BF16, 16, 64, 8, 2, 72), (F16, 33, 12, 3, 3, 96), (BF16, 3, 3, 6, 1, 64)]  # tiles
+
+
+def check_two_parts(dtype, m, n, heads, kv, dim, device):
+    """over few terms probabilities and score gradients enter the products in two 16-bit parts, which leave t^2 of them: results are as far
+    off as their own rounding, t, and 32-bit arithmetic allow"""
+    gen = torch.Generator().manual_seed(17)
+    t = nn_oracle.half_step(dtype)
+    raw = {"q": torch.randn(2, heads, m, dim, generator=gen), "k": torch.randn(2, kv, n, dim, generator=gen), "v": torch.randn(2, kv, n, dim, generator=gen),
+           "grad": torch.randn(2, heads, m, dim, generator=gen)}
+    raw = {k: v.to(dtype) for k, v in raw.items()}
+    table, index = torch.randn(5, heads, generator=gen), torch.randint(0, 5, (m, n), generator=gen)
+    out, (dq, dk, dv) = attention_gradients(raw, RelativeBuckets.from_index(index.to(device)), table, device)
+    group = heads // kv
+    x = attention_64(raw["q"], raw["k"].repeat_interleave(group, 1), raw["v"].repeat_interleave(group, 1), raw["grad"], table[index].movedim(-1, 0))
+    shared = lambda y: y.view(2, kv, group, n, dim).sum(2)                           # noqa: E731
+    smallest = 2.0 ** -25 if dtype == F16 else 0.0
+    terms = m * group * U
+    want = {"out": x["out"], "dq": x["dq"], "dk": shared(x["dk"]), "dv": shared(x["dv"])}
+    bound = {"out": (x["p"] * (x["rel"] + t * t + n * U)) @ x["v"].abs() + t * x["out"].abs(),
+             "dq": dq_bound(x, t, 0.0, t * t),
+             "dk": shared((x["ds_err"] + (t * t + terms) * x["ds"].abs()).transpose(-2, -1) @ x["q"].abs()) * x["scale"] + (t + 2 * U) * want["dk"].abs(),
+             "dv": shared((x["p"] * (x["rel"] + t * t + terms)).transpose(-2, -1) @ x["grad"].abs()) + t * want["dv"].abs()}
+    windows = m <= 64 and n <= 64 and dim <= 64 and heads == kv
+    for name, got in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+        if name == "out" and not windows and m * group > 16:
+            continue                                     # (tiles' forward pass: one part)
+        off = (got.detach().cpu().double() - want[name]).abs()
+        assert (off <= bound[name] + smallest).all(), (name, (off / bound[name]).max())
+
+
+def check_two_parts_token(dtype, n, device):
+    gen = torch.Generator().manual_seed(18)
+    t = nn_oracle.half_step(dtype)
+    q, k, v = (torch.randn(2, h, r, 64, generator=gen).to(dtype) for h, r in ((8, 1), (2, n), (2, n)))
+    table = torch.randn(5, 8, generator=gen)
+    plan = RelativeBuckets.by_distance(torch.arange(5).to(device), -4)
+    out = relative_attention(q.to(device), k.to(device), v.to(device), table.to(device), plan, query_start=n - 1)
+    index = (torch.arange(n) - (n - 1) + 4).clamp(0, 4)[None]
+    x = attention_64(q, k.repeat_interleave(4, 1), v.repeat_interleave(4, 1), torch.zeros_like(q), table[index].movedim(-1, 0))
+    off = (out.cpu().double() - x["out"]).abs()
+    bound = (x["p"] * (x["rel"] + t * t + n * U)) @ x["v"].abs() + t * x["out"].abs() + (2.0 ** -25 if dtype == F16 else 0.0)
+    assert (off <= bound).all(), (off / bound).max()

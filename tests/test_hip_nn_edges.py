@@ -150,3 +150,13 @@ def test_window_transformer_made_in_inference_mode(monkeypatch):
         want = layer(x)
     # both sum some 100 products in 32 bits, in another order
     assert (got - want).abs().max() <= 200 * edges.U * want.abs().max()
+
+
+@pytest.mark.parametrize("dtype,m,n,heads,kv,dim", edges.SHORT)
+def test_two_parts(dtype, m, n, heads, kv, dim):
+    edges.check_two_parts(dtype, m, n, heads, kv, dim, DEV)
+
+
+@pytest.mark.parametrize("dtype,n", [(edges.BF16, 300), (edges.F16, 1500)])
+def test_two_parts_token(dtype, n):
+    edges.check_two_parts_token(dtype, n, DEV)

@@ -188,3 +188,13 @@ def test_plan_of_a_window_transformer():
         if made is torch.no_grad:
             layer.load_state_dict(layer.state_dict())
             assert layer._buckets() is not plan
+
+
+@pytest.mark.parametrize("dtype,m,n,heads,kv,dim", edges.SHORT)
+def test_two_parts(host, dtype, m, n, heads, kv, dim):
+    edges.check_two_parts(dtype, m, n, heads, kv, dim, "cpu")
+
+
+@pytest.mark.parametrize("dtype,n", [(edges.BF16, 300), (edges.F16, 1500)])
+def test_two_parts_token(host, dtype, n):
+    edges.check_two_parts_token(dtype, n, "cpu")

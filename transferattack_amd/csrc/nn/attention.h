@@ -147,19 +147,27 @@ constexpr float kMostLift = 0x1p127f;                    // `up` before the firs
 // ---- products that contract over a tile's rows
 // The weights of one column for 16 SUBS rows, as the matrix instructions take them: fp32 as they are; for 16-bit tensors
 // rounded to their type (an error of half a step per weight, independent from weight to weight, where the result itself is
-// rounded by as much).
+// rounded by as much: results are 1.2 to 1.5 times as far off as their own rounding), or in two parts, which leaves nothing of that.
+// Two parts where they cost little or few terms average little out: single tokens (148 us either way), windows (forward 90 us either
+// way, backward 163 -> 202 us at 32 dims, 150 -> 166 at 64), backward of short rows.  One in the tiles of long rows, whose second
+// products would cost: 8191 tokens of 128 in fp16 428 -> 530 us, and the backward's as attention_bwd.hip says.
 template <class T, int SUBS> struct Weights {
     typename Frag<T>::Row v[SUBS / 2];                   // step s: rows 32 s + 4 g + i and 32 s + 16 + 4 g + i
     __device__ __forceinline__ void from_tiles(const f32x4 (&w)[SUBS]) {
 #pragma unroll
         for (int s = 0; s < SUBS / 2; ++s) v[s] = pack8(w[2 * s], w[2 * s + 1], T{});
     }
-    // from a row of LDS that holds the column's weights by row number
-    __device__ __forceinline__ void from_lds(const T* p, int g) {
+    // what `rounded` lacks of w
+    __device__ __forceinline__ void rest_of(const f32x4 (&w)[SUBS], const Weights& rounded) {
 #pragma unroll
         for (int s = 0; s < SUBS / 2; ++s) {
-            const u16x4 lo = *reinterpret_cast<const u16x4*>(p + 32 * s + 4 * g), hi = *reinterpret_cast<const u16x4*>(p + 32 * s + 16 + 4 * g);
-            v[s] = __builtin_bit_cast(typename Frag<T>::Row, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            f32x4 lo = w[2 * s], hi = w[2 * s + 1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                lo[i] -= static_cast<float>(rounded.v[s][i]);
+                hi[i] -= static_cast<float>(rounded.v[s][4 + i]);
+            }
+            v[s] = pack8(lo, hi, T{});
         }
     }
 };
@@ -168,10 +176,6 @@ template <int SUBS> struct Weights<float, SUBS> {
     __device__ __forceinline__ void from_tiles(const f32x4 (&w)[SUBS]) {
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) v[t] = w[t];
-    }
-    __device__ __forceinline__ void from_lds(const float* p, int g) {
-#pragma unroll
-        for (int t = 0; t < SUBS; ++t) v[t] = *reinterpret_cast<const f32x4*>(p + 16 * t + 4 * g);
     }
 };
 
@@ -212,12 +216,33 @@ __device__ __forceinline__ void mma_transposed(const T* lds, const Weights<T, SU
             }
     }
 }
-template <int DP, int NQ, int SUBS, class T>
+// the same, the first SPLIT of the weights in two 16-bit parts
+template <int DP, int NQ, int SUBS, int SPLIT = 0, class T>
 __device__ __forceinline__ void mma_transposed(const T* lds, const f32x4 (&w)[NQ][SUBS], f32x4 (&acc)[NQ][DP / 16], int c, int g) {
     Weights<T, SUBS> packed[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) packed[q].from_tiles(w[q]);
-    mma_transposed<DP, NQ, SUBS, T>(lds, packed, acc, c, g);
+    if constexpr (SPLIT == 0 || sizeof(T) == 4) {
+        mma_transposed<DP, NQ, SUBS, T>(lds, packed, acc, c, g);
+    } else {
+        Weights<T, SUBS> rest[SPLIT];
+#pragma unroll
+        for (int q = 0; q < SPLIT; ++q) rest[q].rest_of(w[q], packed[q]);
+#pragma unroll
+        for (int s = 0; s < SUBS / 2; ++s)
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                const unsigned short* p = reinterpret_cast<const unsigned short*>(lds) + (32 * s + 4 * g + (c >> 2)) * Tile<T, DP>::LD
+                                          + 16 * dt + 4 * (c & 3);
+                const u16x4 lo = read_transposed(p), hi = read_transposed(p + 16 * Tile<T, DP>::LD);
+                const u16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    acc[q][dt] = mfma(__builtin_bit_cast(typename Frag<T>::Row, a), packed[q].v[s], acc[q][dt]);
+                    if (q < SPLIT) acc[q][dt] = mfma(__builtin_bit_cast(typename Frag<T>::Row, a), rest[q].v[s], acc[q][dt]);
+                }
+            }
+    }
 }
 
 // ---- bias and mask of a score

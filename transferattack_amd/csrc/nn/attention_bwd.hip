@@ -6,7 +6,10 @@
 // (dk, dv), and a tile of pairs stays while the batch streams past it (the table).  No sum crosses workgroups except the
 // table's, whose partial sums a last kernel adds in a fixed order.
 // p and ds are rounded to 16 bits where they enter a 16-bit matrix instruction: half a step of each term (in fp16 brought into its
-// range before, see attention.h).
+// range before, see attention.h), which makes gradients about sqrt(2) of the rounding of their results off.  Over few terms -- calls of
+// up to 64 keys, or of 64 queries times the heads that share a key head -- it is up to 1.9 of it, and there both enter in two parts (1.0).
+// Over many that would cost 251 instead of 233 us (64 x 12 x 196 tokens, all gradients and the forward pass) and 313 instead of 280
+// (8 x 12 x 1023).
 // Together 9 products of m n dim, the forward's two aside, where 5 are needed: scores and dp are computed once for each kernel
 // rather than 16-bit sums exchanged through atomics, whose order would change results.  Bound like the forward by LDS reads and
 // issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 74 us, keys 87, table 42 + 20 (near tiles only: what is
@@ -16,7 +19,9 @@
 
 namespace ta_nn {
 
-template <class T, int DP, int BIASES>
+constexpr int kFewTerms = 64;                            // of a sum over keys, or over queries and the heads that share a key head
+
+template <class T, int DP, int BIASES, int FEW>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_q(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = sizeof(T) == 2 ? 2 : kSubs<DP>, ROWS = 16 * SUBS;
     constexpr int SUMS = sizeof(T) == 2 ? 2 : 1;         // of ds k, and of p k for the correction below
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
                 far_dp[1] += end > 0 ? exact_tile : 0.0f;
             }
         }
-        mma_transposed<DP, SUMS, SUBS>(ks, ds, dq, c, g);
+        mma_transposed<DP, SUMS, SUBS, FEW>(ks, ds, dq, c, g);
         });
     }
     exact = reduce_rows(exact, Sum{});
@@ -164,7 +169,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
     if (valid) store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + head * a.dq_sh + query * a.dq_sm, dq[0], a.scale, a.dim, g);
 }
 
-template <class T, int DP, int BIASES>
+template <class T, int DP, int BIASES, int FEW>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attention_bwd_kv(AttentionArgs a) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, SUBS = sizeof(T) == 2 ? 2 : kSubs<DP>, ROWS = 16 * SUBS;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -267,8 +272,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void atten
             }
         }
         if constexpr (kNarrow<T>) into_range(ds[0], dk[0], up);
-        mma_transposed<DP, 1, SUBS>(gs, p, dv, c, g);
-        mma_transposed<DP, 1, SUBS>(qs, ds, dk, c, g);
+        mma_transposed<DP, 1, SUBS, FEW>(gs, p, dv, c, g);
+        mma_transposed<DP, 1, SUBS, FEW>(qs, ds, dk, c, g);
         });
     }
     if (!used) {
@@ -495,8 +500,18 @@ template <class T, int DP> int launch_backward(AttentionArgs a, hipStream_t st) 
     const int64_t q_blocks = ceil_div(a.m, 64) * a.heads * a.batch, k_blocks = ceil_div(a.n, 64) * a.kv_heads * a.batch;
     const int64_t t_blocks = ceil_div(a.m, 64) * (a.distances ? near_tiles(a) : ceil_div(a.n, 64)) * a.heads * a.chunks;
     TA_NN_REQUIRE(q_blocks <= 0x7FFFFFFF && k_blocks <= 0x7FFFFFFF && t_blocks <= 0x7FFFFFFF, "too many tokens for one launch");
-    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_q<T, DP, BIASES>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a));
-    TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_kv<T, DP, BIASES>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), tiles + 3 * 64 * 4 + bias, st, a));
+    // (short calls have one instance, the one that takes any bias)
+    if (sizeof(T) == 2 && a.n <= kFewTerms) {
+        hipLaunchKernelGGL((attention_bwd_q<T, DP, kAny, sizeof(T) == 2>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a);
+    } else {
+        TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_q<T, DP, BIASES, 0>), dim3(static_cast<unsigned>(q_blocks)), dim3(256), tiles + bias, st, a));
+    }
+    const size_t kv_lds = tiles + 3 * 64 * 4 + bias;
+    if (sizeof(T) == 2 && static_cast<int64_t>(a.m) * (a.heads / a.kv_heads) <= kFewTerms) {
+        hipLaunchKernelGGL((attention_bwd_kv<T, DP, kAny, sizeof(T) == 2>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), kv_lds, st, a);
+    } else {
+        TA_NN_BY_BIASES(a, hipLaunchKernelGGL((attention_bwd_kv<T, DP, BIASES, 0>), dim3(static_cast<unsigned>(k_blocks)), dim3(256), kv_lds, st, a));
+    }
     if (a.dtable) {
         const size_t diagonals = 64 * 65 * 4;
         const size_t lds = table_tiles + bias > diagonals ? table_tiles + bias : diagonals;

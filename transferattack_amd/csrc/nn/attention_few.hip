@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256, 2) void attention_few(AttentionArgs a, int chu
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[0][dt] *= shrink;
         wave_lds_order();                                // (the wave's own rows: its LDS operations are done in order)
-        mma_transposed<DP, 1, SUBS>(vs, s, o, c, g);
+        mma_transposed<DP, 1, SUBS, 1>(vs, s, o, c, g);
         wave_lds_order();
     }
     l = reduce_rows(l, Sum{});

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void window_fwd(AttentionArgs a, int parts)
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        mma_transposed<DP, 1, 4>(vs, s, o, c, g);
+        mma_transposed<DP, 1, 4, 1>(vs, s, o, c, g);
         if (valid) {
             const int64_t b = share.sequence(i);
             store_column<T, DP>(static_cast<T*>(a.out) + b * a.o_sb + share.head * a.o_sh + query * a.o_sm, o[0], inv, a.dim, g);
@@ -135,16 +135,14 @@ __global__ __launch_bounds__(256, 2) void window_fwd(AttentionArgs a, int parts)
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts) {
     constexpr int DC = DP / Frag<T>::D, DT = DP / 16, TILE = 64 * Tile<T, DP>::LD;
-    constexpr int WLD = 64 + 16 / static_cast<int>(sizeof(T));       // rows of the transposed weights, [key][query]
+    constexpr int WLD = 64 + 4;                          // rows of the transposed weights, [key][query], in 32 bits
     extern __shared__ __attribute__((aligned(16))) char smem[];
     T* ks = reinterpret_cast<T*>(smem);
     T* vs = ks + TILE;
     T* qs = vs + TILE;
     T* gs = qs + TILE;
-    T* ps = gs + TILE;
-    T* dss = ps + 64 * WLD;                              // fp16: in 32 bits, until the column's largest is known
-    constexpr int FLD = 64 + 4;
-    float* dss32 = reinterpret_cast<float*>(dss);
+    float* ps = reinterpret_cast<float*>(gs + TILE);
+    float* dss = ps + 64 * WLD;
     constexpr float LIFT = 1 << kLift<T>;
     const int tid = threadIdx.x, wave = tid >> 6, c = tid & 15, g = (tid >> 4) & 3;
     const Share share(a, parts);
@@ -212,9 +210,8 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
                     const float w = p[t][r];
                     ds[0][t][r] = w * (ds[0][t][r] - delta);
                     table_sum[t][r] += ds[0][t][r];
-                    ps[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(w * LIFT);
-                    if constexpr (kNarrow<T>) dss32[(16 * t + 4 * g + r) * FLD + own] = ds[0][t][r];
-                    else dss[(16 * t + 4 * g + r) * WLD + own] = from_float<T>(ds[0][t][r]);
+                    ps[(16 * t + 4 * g + r) * WLD + own] = w * LIFT;
+                    dss[(16 * t + 4 * g + r) * WLD + own] = ds[0][t][r];
                 }
         }
         {
@@ -223,29 +220,24 @@ __global__ __launch_bounds__(256, 2) void window_bwd(AttentionArgs a, int parts)
             for (int dt = 0; dt < DT; ++dt) dq[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             float up = kNarrow<T> ? kMostLift : 1.0f;
             if constexpr (kNarrow<T>) into_range(ds[0], dq[0], up);
-            mma_transposed<DP, 1, 4>(ks, ds, dq, c, g);
+            mma_transposed<DP, 1, 4, 1>(ks, ds, dq, c, g);
             if (own < a.m)
                 store_column<T, DP>(static_cast<T*>(a.dq) + b * a.dq_sb + share.head * a.dq_sh + own * a.dq_sm, dq[0], a.scale * (1.0f / up), a.dim, g);
         }
         __syncthreads();
         {
             f32x4 dk[1][DT], dv[1][DT];
-            Weights<T, 4> w[1];
+            f32x4 w[1][4];
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) dk[0][dt] = dv[0][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            w[0].from_lds(ps + own * WLD, g);
-            mma_transposed<DP, 1, 4>(gs, w, dv, c, g);
-            float up = kNarrow<T> ? kMostLift : 1.0f;
-            if constexpr (kNarrow<T>) {
-                f32x4 column[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) column[t] = *reinterpret_cast<const f32x4*>(dss32 + own * FLD + 16 * t + 4 * g);
-                into_range(column, dk[0], up);
-                w[0].from_tiles(column);
-            } else {
-                w[0].from_lds(dss + own * WLD, g);
-            }
-            mma_transposed<DP, 1, 4>(qs, w, dk, c, g);
+            for (int t = 0; t < 4; ++t) w[0][t] = *reinterpret_cast<const f32x4*>(ps + own * WLD + 16 * t + 4 * g);
+            mma_transposed<DP, 1, 4, 1>(gs, w, dv, c, g);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[0][t] = *reinterpret_cast<const f32x4*>(dss + own * WLD + 16 * t + 4 * g);
+            float up = kNarrow<T> ? kMostLift : 1.0f;
+            if constexpr (kNarrow<T>) into_range(w[0], dk[0], up);
+            mma_transposed<DP, 1, 4, 1>(qs, w, dk, c, g);
             if (own < a.n) {
                 store_column<T, DP>(static_cast<T*>(a.dk) + b * a.dk_sb + share.head * a.dk_sh + own * a.dk_sn, dk[0], a.scale * (1.0f / up), a.dim, g);
                 store_column<T, DP>(static_cast<T*>(a.dv) + b * a.dv_sb + share.head * a.dv_sh + own * a.dv_sn, dv[0], 1.0f / LIFT, a.dim, g);
@@ -278,8 +270,7 @@ template <class T, int DP> int launch_window_by(AttentionArgs a, bool backward, 
         hipLaunchKernelGGL((window_fwd<T, DP>), dim3(static_cast<unsigned>(blocks)), dim3(256), 4 * tile, st, a, parts);
         return check_launch("ta_nn_attention");
     }
-    const size_t weights = 64 * (64 + 16 / sizeof(T)) * sizeof(T), diagonals = 64 * 65 * 4;
-    const size_t lds = 4 * tile + weights + (kNarrow<T> ? 64 * (64 + 4) * 4 : weights);
+    const size_t lds = 4 * tile + 2 * 64 * (64 + 4) * 4, diagonals = 64 * 65 * 4;
     hipLaunchKernelGGL((window_bwd<T, DP>), dim3(static_cast<unsigned>(blocks)), dim3(256), lds > diagonals ? lds : diagonals, st, a, parts);
     return check_launch("ta_nn_attention_backward");
 }
