@@ -587,3 +587,20 @@ def check_two_parts_token(dtype, n, device):
     off = (out.cpu().double() - x["out"]).abs()
     bound = (x["p"] * (x["rel"] + t * t + n * U)) @ x["v"].abs() + t * x["out"].abs() + (2.0 ** -25 if dtype == F16 else 0.0)
     assert (off <= bound).all(), (off / bound).max()
+
+
+def check_temperatures(device):
+    """temperatures whose reciprocal 32 bits do not hold are refused; the outermost others give a distribution: the hottest all classes alike,
+    the coldest the largest alone"""
+    x, classes = torch.tensor([[3.0, -torch.inf, 1.0, 2.0, 2.5]]), torch.tensor([[0, 3]])
+    for t in (2.0 ** -127, 1e-46, 2.0 ** 127, 1e300, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            top_logits(x.to(device), 2, temperature=t)
+        with pytest.raises(ValueError, match="temperature"):
+            TopLogits(x[:, :2].to(device), classes.to(device), None, t)
+    hot, cold = top_logits(x.to(device), 2, temperature=2.0 ** 126), top_logits(x.to(device), 2, temperature=2.0 ** -100)
+    assert abs(float(hot.rest) - float(torch.tensor(2.0).log())) <= 4 * U and float(cold.rest) == 2.0 ** 101
+    for t in (2.0 ** 30, 2.0 ** -100):
+        answers = TopLogits(torch.tensor([[3.0, 2.0]]).to(device), classes.to(device), None, t)
+        loss, grad = distillation_loss_and_grad(x.to(device), answers, reduction="sum")
+        assert torch.isfinite(loss) and torch.isfinite(grad).all() and float(grad[0, 1].abs()) == 0.0

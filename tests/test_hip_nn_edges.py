@@ -160,3 +160,7 @@ def test_two_parts(dtype, m, n, heads, kv, dim):
 @pytest.mark.parametrize("dtype,n", [(edges.BF16, 300), (edges.F16, 1500)])
 def test_two_parts_token(dtype, n):
     edges.check_two_parts_token(dtype, n, DEV)
+
+
+def test_temperatures():
+    edges.check_temperatures(DEV)

@@ -198,3 +198,7 @@ def test_two_parts(host, dtype, m, n, heads, kv, dim):
 @pytest.mark.parametrize("dtype,n", [(edges.BF16, 300), (edges.F16, 1500)])
 def test_two_parts_token(host, dtype, n):
     edges.check_two_parts_token(dtype, n, "cpu")
+
+
+def test_temperatures(host):
+    edges.check_temperatures("cpu")

@@ -715,13 +715,16 @@ template <class T> int launch_top(const TopArgs& a, int64_t rows, hipStream_t st
     return check_launch("ta_nn_top_logits");
 }
 
+// log2 e / T is an ordinary number of 32 bits, so that it times a difference of 0 or -inf is what it should be
+static bool temperature_in_range(double t) { return t >= 0x1p-126 && t <= 0x1p126; }
+
 static int check_rows(const DistilArgs& a, int64_t rows) {
     TA_NN_REQUIRE(a.x && a.top_values && a.top_classes, "null pointer");
     TA_NN_REQUIRE(rows >= 1 && rows <= 0x7FFFFFFF, "rows %lld", static_cast<long long>(rows));
     TA_NN_REQUIRE(a.classes >= 1 && a.classes <= kMaxClasses, "classes %d (1 .. %d)", a.classes, kMaxClasses);
     TA_NN_REQUIRE(a.k >= 1 && a.k <= kMaxTop, "top classes %d (1 .. %d)", a.k, kMaxTop);
     TA_NN_REQUIRE(a.x_stride >= a.classes, "row stride %lld of %d classes", static_cast<long long>(a.x_stride), a.classes);
-    TA_NN_REQUIRE(a.temperature > 0.0 && a.temperature < INFINITY, "temperature %g", a.temperature);
+    TA_NN_REQUIRE(temperature_in_range(a.temperature), "temperature %g (2^-126 .. 2^126)", a.temperature);
     return 0;
 }
 
@@ -744,7 +747,7 @@ extern "C" int ta_nn_top_logits(const void* x, int dtype, int64_t x_stride, int6
     TA_NN_REQUIRE(classes >= 1 && classes <= (1 << 30) && x_stride >= classes, "%d classes (1 .. 2^30), row stride %lld", classes,
                   static_cast<long long>(x_stride));
     TA_NN_REQUIRE(k >= 1 && k <= classes && k <= ta_nn::kMaxTop, "%d of %d classes (at most %d)", k, classes, ta_nn::kMaxTop);
-    TA_NN_REQUIRE(temperature > 0.0f && temperature < INFINITY, "temperature %g", static_cast<double>(temperature));
+    TA_NN_REQUIRE(ta_nn::temperature_in_range(temperature), "temperature %g (2^-126 .. 2^126)", static_cast<double>(temperature));
     const ta_nn::TopArgs a{x, x_stride, classes, k, temperature, values, top_classes, rest};
     TA_NN_BY_TYPE(dtype, ta_nn::launch_top<T>(a, rows, static_cast<hipStream_t>(stream)));
 }

@@ -39,7 +39,7 @@ class TopLogits:
             raise ValueError("rest must be float32 [rows]")
         if classes.device != values.device or (rest is not None and rest.device != values.device):
             raise ValueError("values, classes and rest must be on one device")
-        if not 0.0 < float(temperature) < float("inf"):
+        if not 2.0 ** -126 <= float(temperature) <= 2.0 ** 126:
             raise ValueError("temperature %r" % (temperature,))
         if not 1 <= values.shape[1] <= MAX_TOP:
             raise ValueError("%d classes answered (1 .. %d)" % (values.shape[1], MAX_TOP))
@@ -98,7 +98,7 @@ def top_logits(logits, top, temperature=1.0, rest=True):
     rows = _rows_of(logits.detach() if isinstance(logits, torch.Tensor) else logits)
     if not 1 <= top <= min(rows.shape[1], MAX_TOP):
         raise ValueError("top %r of %d classes (at most %d)" % (top, rows.shape[1], MAX_TOP))
-    if not 0.0 < float(temperature) < float("inf"):
+    if not 2.0 ** -126 <= float(temperature) <= 2.0 ** 126:
         raise ValueError("temperature %r" % (temperature,))
     n = rows.shape[0]
     values = torch.empty((n, top), dtype=torch.float32, device=rows.device)
