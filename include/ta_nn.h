@@ -68,8 +68,8 @@ typedef struct ta_nn_attention_args {
     int start, causal;                           /* causal: key j is seen if j <= start + i */
     void* out;
     int64_t o_sb, o_sh, o_sm;
-    float* stats;                                /* [batch][heads][m][2]: maximum of the scores and 1 / sum of the exponentials,
-                                                    for a backward pass; or NULL */
+    float* stats;                                /* [batch][heads][m][2]: a score near the largest and 1 / sum of the exponentials
+                                                    relative to it, for a backward pass; or NULL */
     float* workspace;                            /* ta_nn_attention_workspace() floats, or NULL where that is 0 */
     /* backward: */
     const void* grad;                            /* of out; out and stats are the forward pass's */

@@ -10,11 +10,12 @@
 // up to 64 keys, or of 64 queries times the heads that share a key head -- it is up to 1.9 of it, and there both enter in two parts (1.0).
 // Over many that would cost 251 instead of 233 us (64 x 12 x 196 tokens, all gradients and the forward pass) and 313 instead of 280
 // (8 x 12 x 1023).
-// Together 9 products of m n dim, the forward's two aside, where 5 are needed: scores and dp are computed once for each kernel
-// rather than 16-bit sums exchanged through atomics, whose order would change results.  Bound like the forward by LDS reads and
-// issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 74 us, keys 87, table 42 + 20 (near tiles only: what is
-// past an end of the distances is summed by the queries' kernel, which meets those pairs anyway); 64 x 12 x 196 tokens in pairs,
-// 50, 57, 59 + 15 us.  64-row tiles (two waves to a SIMD) instead of 32: 81 and 105 us for the first two.
+// Together 9 products of m n dim, the forward's two aside, where 5 are needed (16-bit types: 10, with dq's correction): scores and dp
+// are computed once for each kernel, since dq and dk, dv sum over different sides of the same scores.  Bound like the forward by LDS
+// reads and issue.  Measured, bf16, heads of 64: 8 x 12 x 1023 padded tokens, queries 80 us (74 without the correction), keys 87,
+// table 42 + 20 (near tiles only: what is past an end of the distances is summed by the queries' kernel, which meets those pairs
+// anyway); 64 x 12 x 196 tokens in pairs, 52, 57, 60 + 15 us.  64-row tiles (two waves to a SIMD) instead of 32: 81 and 105 us for the
+// first two, against 71 and 91 at the time.
 #include "attention.h"
 
 namespace ta_nn {
@@ -416,7 +417,7 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v)
 }
 
 // Pairs, first: the chunks' sums of every pair, 64 pairs to a workgroup, its four waves a quarter of the chunks each; 64-bit sums,
-// written in two halves over the first chunk's place.  (Reading them bucket by bucket instead touches a line for every value.)
+// rounded to 32 bits over the first chunk's place.  (Reading them bucket by bucket instead touches a line for every value.)
 __global__ __launch_bounds__(256) void attention_pair_sums(AttentionArgs a) {
     __shared__ double red[4][64];
     const int64_t pairs = static_cast<int64_t>(a.m) * a.n, tiles = (pairs + 63) / 64;

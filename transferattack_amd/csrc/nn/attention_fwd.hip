@@ -9,8 +9,8 @@ template <class T> constexpr float kBelow = kNarrow<T> ? 15.0f - kSlack : 0.0f; 
 // One workgroup: 64 NQ columns (queries; those of all heads that share a key head in one row, so that shared heads share the
 // tiles) against every key they see, a tile at a time.  Two tiles in LDS: while one is worked on, the next arrives in registers
 // and is put into the other's place, with one barrier a tile.  Bound by LDS reads and by issue (16 columns to a wave: a byte of LDS
-// for every 32 operations; one exponential and a few fp32 operations a score), not by memory: 16 x 8191 causal tokens of 128 in
-// fp16, 4 key heads, 435 us = 630 Tflop/s of the 1310 a large matrix product reaches; 8 x 12 x 1023 padded tokens of 64 in bf16 52 us.
+// for every 16 operations; one exponential and a few fp32 operations a score), not by memory: 16 x 8191 causal tokens of 128 in
+// fp16, 4 key heads, 430 us = 640 Tflop/s of the 1310 a large matrix product reaches; 8 x 12 x 1023 padded tokens of 64 in bf16 52 us.
 // Three waves to a SIMD for 16-bit types although wide heads then spill a few registers outside the loop: 507 against 511 us.
 template <class T, int DP, int NQ, int BIASES>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && NQ == 1 ? 3 : 2) void attention_fwd(AttentionArgs a) {

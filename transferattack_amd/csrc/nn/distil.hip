@@ -454,7 +454,7 @@ __device__ __forceinline__ float value_of_order(unsigned o) {          // the in
 // bisection over its 64 bits, reading the row again for each.
 // In the common case an element is looked at twice in registers: for its vector's maximum and for its exponential.  Vectors that
 // reach the limit, one or two for each of the K, are copied to LDS and leave the row; their elements get a thread each.
-// Measured: 64 of 65536 bf16, 4096 rows, 170 us (3.1 TB/s: vector units and the first wave's ranking, several rows to a CU at
+// Measured: 64 of 65536 bf16, 4096 rows, 174 us (3.1 TB/s: vector units and the first wave's ranking, several rows to a CU at
 // different stages); 5 of 1000 fp32, 32 rows, 5.6 us, most of it the launch and one row's chain of dependent steps.
 template <class T, int THREADS, int VPT>
 __global__ __launch_bounds__(THREADS, 4) void top_logits(TopArgs a) {

@@ -185,7 +185,8 @@ def distillation_loss(logits, answers, weight=None, reduction="mean"):
     """T^2 KL(teacher || student) of every row at the answers' temperature T, differentiable in the student's ``logits``
     [..., classes] (fp32, bf16 or fp16; rows in the order of the answers').
 
-    weight     fp32, one for each row, or None; a row of weight 0 is not looked at (padding may hold anything)
+    weight     fp32, one for each row, or None; a row of weight 0 is not looked at (padding may hold anything).  Weights and answers have
+               no gradient, and must not change before a backward pass
     reduction  'mean': sum of weight * loss / sum of weights (0 if no row counts); 'sum'; 'none': weight * loss for each row
     The loss is fp32, the gradient has the logits' type."""
     rows = _rows_of(logits)

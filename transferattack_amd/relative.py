@@ -7,7 +7,8 @@ The window transformer the reference evaluates on (transferattack/utils.py:16-17
 windows, a bucket for each 2-D offset; sequence models use logarithmic distance buckets.  ``RelativeBuckets`` is the plan that
 says which bucket a pair has -- built once, like the module's ``relative_position_index`` buffer -- ``relative_attention`` the
 operator, ``relative_attention_packed`` the same on a projection's output as it lies in memory.  Both have a backward pass
-(queries, keys, values, table) and take single tokens against a long cache; neither writes scores to memory.
+(queries, keys, values, table) and take single tokens against a long cache.  No scores are written to memory; the table's gradient
+takes partial sums of their gradients, [parts, heads, m, n] for pairs, and with a mask for every sequence a part is a sequence.
 
 No fallback: tensors must be on a HIP device."""
 import torch
@@ -326,7 +327,8 @@ def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=Fa
     mask         bool (True: may be seen) or additive, [m, n], [period, m, n] or [period, heads, m, n] with 1 for a dimension it
                  does not depend on; sequence b takes mask b % period (windows of an image).  No gradient.
     causal       key j is seen by queries at positions >= j
-    key_lengths  [batch] keys in use; what lies behind them is not read and its gradients are 0
+    key_lengths  [batch] keys in use; what lies behind them is not read and its gradients are 0.  (This, the mask and query_start must
+                 not change before a backward pass: autograd raises if they do)
     query_start  position of query 0 (an int, or [batch] tensor): query i stands at query_start + i, key j at j
     A query that sees no key gives zeros and takes no gradient.  Keys that only a mask hides have to be finite (0 * inf is
     NaN); those past ``key_lengths`` may hold anything.  The table's gradient with distance buckets needs an int ``query_start``.
