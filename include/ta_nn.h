@@ -14,7 +14,7 @@
  *   - element types: TA_NN_F32 / _BF16 / _F16; strides count elements; the innermost dimension is contiguous;
  *   - sums, maxima, softmax statistics and gradients are accumulated in fp32 or fp64 whatever the tensors' type;
  *   - return value: 0, a hipError_t (> 0) or TA_NN_EINVAL (-1); ta_nn_last_error() has the calling thread's last message;
- *   - results are deterministic: no floating-point atomics, every reduction has a fixed order.
+ *   - results are deterministic: no floating-point atomics, every reduction has a fixed order or is exact.
  */
 #ifndef TA_NN_H
 #define TA_NN_H
