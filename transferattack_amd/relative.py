@@ -109,23 +109,13 @@ def _check_buckets(t, dims, name):
 
 # ------------------------------------------------------------------------------------------------------------ the call
 class _Call:
-    """one call's options, checked"""
-    __slots__ = ("buckets", "scale", "mask", "causal", "lengths", "start", "start_tensor")
+    """one call's options, checked; `tensors` are (mask, key lengths, query starts), each a tensor or None"""
+    __slots__ = ("buckets", "scale", "causal", "start", "tensors")
 
-    def __init__(self):
-        self.mask = self.lengths = self.start_tensor = None
-
-    def split(self):
-        """(the options without their tensors, the tensors): a backward pass keeps the latter as autograd keeps inputs, so that one
-        changed in between is an error"""
-        o = _Call()
-        o.buckets, o.scale, o.causal, o.start = self.buckets, self.scale, self.causal, self.start
-        return o, (self.mask, self.lengths, self.start_tensor)
-
-    def joined(self, tensors):
-        o = self.split()[0]
-        o.mask, o.lengths, o.start_tensor = tensors
-        return o
+    def keep(self):
+        """the tensors, for ``save_for_backward``: changed before the backward pass they are an error, so no one else holds them"""
+        tensors, self.tensors = self.tensors, None
+        return _nn.kept(*tensors)
 
 
 def _int32(t, low, high):
@@ -152,6 +142,7 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
     o = _Call()
     o.buckets, o.causal = buckets, bool(causal)
     o.scale = dim ** -0.5 if scale is None else float(scale)
+    view = lengths = starts = None
     if mask is not None:
         _nn.check_tensor(mask, "mask", q, FLOATS + (torch.bool,))
         if mask.requires_grad:
@@ -162,26 +153,27 @@ def _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start
         p, h, i, j = view.shape
         if p == 0 or batch % p or h not in (1, heads) or i not in (1, m) or j not in (1, n):
             raise ValueError("mask %s does not fit batch %d, %d heads, %d queries, %d keys" % (tuple(mask.shape), batch, heads, m, n))
-        o.mask = view
     if key_lengths is not None:
         _nn.check_tensor(key_lengths, "key_lengths", q, (torch.int32, torch.int64))
         if key_lengths.shape != (batch,):
             raise ValueError("key_lengths must be [%d], got %s" % (batch, tuple(key_lengths.shape)))
-        o.lengths = _int32(key_lengths, 0, n)
+        lengths = _int32(key_lengths, 0, n)
     o.start = 0
     if isinstance(query_start, torch.Tensor):
         _nn.check_tensor(query_start, "query_start", q, (torch.int32, torch.int64))
         if query_start.shape != (batch,):
             raise ValueError("query_start must be an int or [%d], got %s" % (batch, tuple(query_start.shape)))
-        o.start_tensor = _int32(query_start, -(1 << 31) + 1, (1 << 31) - 1)
+        starts = _int32(query_start, -(1 << 31) + 1, (1 << 31) - 1)
     else:
         o.start = int(query_start)
         if abs(o.start) >= 1 << 30:
             raise ValueError("query_start %d" % o.start)
+    o.tensors = view, lengths, starts
     return o
 
 
-def _arguments(q, k, v, table, out, stats, o):
+def _arguments(q, k, v, table, out, stats, o, tensors):
+    mask, lengths, starts = tensors
     a = _nn.AttentionArgs()
     a.dtype, a.batch, a.heads, a.m, a.dim = _nn.DTYPES[q.dtype], q.shape[0], q.shape[1], q.shape[2], q.shape[3]
     a.kv_heads, a.n = k.shape[1], k.shape[2]
@@ -195,12 +187,12 @@ def _arguments(q, k, v, table, out, stats, o):
     a.distances, a.first, a.index = b.distances, b.first, b.index.data_ptr()
     if b.index_t is not None:
         a.index_t, a.index_stride, a.index_t_stride = b.index_t.data_ptr(), b.index.stride(0), b.index_t.stride(0)
-    if o.mask is not None:
-        a.mask = o.mask.data_ptr()
-        a.mask_kind = _nn.MASK_BOOL if o.mask.dtype == torch.bool else _nn.MASK_FLOAT + _nn.DTYPES[o.mask.dtype]
-        a.mask_period = o.mask.shape[0]
-        a.mask_sb, a.mask_sh, a.mask_sm, a.mask_sn = [0 if size == 1 else stride for size, stride in zip(o.mask.shape, o.mask.stride())]
-    a.key_lengths, a.query_start, a.start, a.causal = _nn.ptr(o.lengths), _nn.ptr(o.start_tensor), o.start, int(o.causal)
+    if mask is not None:
+        a.mask = mask.data_ptr()
+        a.mask_kind = _nn.MASK_BOOL if mask.dtype == torch.bool else _nn.MASK_FLOAT + _nn.DTYPES[mask.dtype]
+        a.mask_period = mask.shape[0]
+        a.mask_sb, a.mask_sh, a.mask_sm, a.mask_sn = [0 if size == 1 else stride for size, stride in zip(mask.shape, mask.stride())]
+    a.key_lengths, a.query_start, a.start, a.causal = _nn.ptr(lengths), _nn.ptr(starts), o.start, int(o.causal)
     a.stats = _nn.ptr(stats)
     return a
 
@@ -222,14 +214,14 @@ def _forward(q, k, v, table, out, o, save):
     if k.shape[2] == 0:
         out.zero_()
         return stats
-    a = _arguments(q, k, v, table, out, stats, o)
+    a = _arguments(q, k, v, table, out, stats, o, o.tensors)
     ws = _workspace(a, q, False)                         # kept alive until the launches are enqueued
     _nn._launch("ta_nn_attention", q, a)
     del ws
     return stats
 
 
-def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
+def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o, tensors):
     dtable = None
     if table_grad:                                       # rows behind the plan's last bucket are not written
         covered = table.shape[0] == o.buckets.buckets and out.numel() > 0 and k.shape[2] > 0
@@ -239,7 +231,7 @@ def _backward(q, k, v, table, out, stats, grad, dq, dk, dv, table_grad, o):
             t.zero_()
         return dtable
     grad = _dense_rows(grad)
-    a = _arguments(q, k, v, table, out, stats, o)
+    a = _arguments(q, k, v, table, out, stats, o, tensors)
     a.grad = grad.data_ptr()
     a.g_sb, a.g_sh, a.g_sm, _ = grad.stride()
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
@@ -265,8 +257,8 @@ class _RelativeAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, table, o):
         out = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
         stats = _forward(q, k, v, table, out, o, True)
-        ctx.options, tensors = o.split()
-        ctx.save_for_backward(q, k, v, table, out, stats, *_nn.kept(*tensors))
+        ctx.options = o
+        ctx.save_for_backward(q, k, v, table, out, stats, *o.keep())
         return out
 
     @staticmethod
@@ -276,7 +268,7 @@ class _RelativeAttention(torch.autograd.Function):
         dq = _token_major(q.shape[0], q.shape[1], q.shape[2], q.shape[3], q)
         dk = _token_major(k.shape[0], k.shape[1], k.shape[2], k.shape[3], k)
         dv = _token_major(v.shape[0], v.shape[1], v.shape[2], v.shape[3], v)
-        dtable = _backward(q, k, v, table, out, stats, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options.joined(tensors))
+        dtable = _backward(q, k, v, table, out, stats, grad, dq, dk, dv, ctx.needs_input_grad[3], ctx.options, tensors)
         return dq, dk, dv, dtable, None
 
 
@@ -291,8 +283,8 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, table, o):
         out, stats = _packed_forward(qkv, table, o, True)
-        ctx.options, tensors = o.split()
-        ctx.save_for_backward(qkv, table, out, stats, *_nn.kept(*tensors))
+        ctx.options = o
+        ctx.save_for_backward(qkv, table, out, stats, *o.keep())
         return out.flatten(2)
 
     @staticmethod
@@ -303,7 +295,7 @@ class _PackedAttention(torch.autograd.Function):
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         dq, dk, dv = dqkv.permute(2, 0, 3, 1, 4).unbind(0)
         grad = grad.reshape(out.shape).transpose(1, 2)
-        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options.joined(tensors))
+        dtable = _backward(q, k, v, table, out.transpose(1, 2), stats, grad, dq, dk, dv, ctx.needs_input_grad[1], ctx.options, tensors)
         return dqkv, dtable, None
 
 
@@ -344,7 +336,7 @@ def relative_attention(q, k, v, table, buckets, scale=None, mask=None, causal=Fa
     o = _options(q, k, table, buckets, scale, mask, causal, key_lengths, query_start)
     _nn.no_tangents(q, k, v, table, mask)
     save = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)
-    if save and table.requires_grad and o.start_tensor is not None and buckets.distances:
+    if save and table.requires_grad and o.tensors[2] is not None and buckets.distances:
         raise ValueError("the table's gradient needs one query_start for all sequences (an int)")
     dim, pad = q.shape[3], _padding(q)
     if pad:
