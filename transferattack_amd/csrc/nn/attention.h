@@ -115,7 +115,8 @@ __device__ __forceinline__ half8 pack8(f32x4 a, f32x4 b, fp16) {
 }
 // ---- fp16's range: 11 bits from 2^-14 up to 65504.  Probabilities are multiplied by 2^kLift before they are rounded (so down to 2^-26
 // of 1 keep their bits, and even scores that the passes make 2.7 apart do not overflow), score gradients, which may have any size, by a
-// power of two for each column that brings the largest so far to 2^11 .. 2^15.  All exact, and taken out of the sums again.
+// power of two for each column that brings the largest so far to 2^11 .. 2^15.  All exact, and taken out of the sums again.  It costs
+// the queries' and the keys' kernel some 10 % each (8 x 12 x 1023 padded tokens of 64, step in fp16 320 us; bf16 281).
 template <class T> constexpr bool kNarrow = Frag<T>::NARROW;
 template <class T> constexpr int kLift = kNarrow<T> ? 12 : 0;
 template <int SUBS> __device__ __forceinline__ float peak_of(const f32x4 (&w)[SUBS]) {      // of a column, over its four lanes (NaN aside)
